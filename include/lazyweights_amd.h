@@ -205,6 +205,76 @@ long long lw_build_layout(const uint8_t* blob, long long len, int N, int KS, int
                           uint16_t* mid, uint16_t* split, uint16_t* rows, uint64_t* sched, int* ring_rows,
                           uint32_t* words, long long words_cap);
 
+/* ── attention over a paged key-value cache (extensions: the reference keeps one contiguous fp16 cache inside its model
+ * runtime, kernels/llmrt.cu:1305-1497) ──────────────────────────────────────────────────────────────────────── */
+
+/* Element types of activations, caches and outputs. */
+enum { LW_F32 = 0, LW_F16 = 1, LW_BF16 = 2 };
+
+/* A caller-owned cache on the GPU: row r of page p of key-value head h starts at k (v) + p * page_stride + h * head_stride +
+ * r * row_stride elements of `type` (LW_F16 or LW_BF16) and holds head_dim contiguous elements (64, 96 or 128). Pages of
+ * page_size rows, a power of two up to 65536; strides are multiples of 8 elements, k and v aligned to 16 bytes. */
+typedef struct lw_kv_cache {
+  void* k;
+  void* v;
+  int64_t pages, page_stride, head_stride, row_stride;
+  int32_t page_size, kv_heads, head_dim, type;
+} lw_kv_cache;
+
+/* A batch of sequences, its arrays on the GPU. Row t (a new token; `tokens` of them) belongs to the sequence s with
+ * q_start[s] <= t < q_start[s + 1]; a sequence's rows are its last positions, so t has position
+ * kv_len[s] - q_start[s + 1] + t, and kv_len[s] counts them. Position j lies in row j % page_size of page
+ * page_table[s * table_stride + j / page_size]. Sequences may have no rows and no length. max_new and max_kv bound the
+ * rows and the length of every sequence; launches are sized by them, so that the arrays can change between calls (and
+ * between replays of a captured call) without the host reading them. What the arrays hold is kept in range by the
+ * kernels: rows lie in [0, tokens), lengths in the page table, and a page number outside [0, pages) stands for a page
+ * that is not there: nothing is appended to it and no row sees its positions. workspace: lw_attn_workspace() bytes,
+ * aligned to 16, zero before its first use; calls leave it ready for the next one. Calls that share one must not
+ * overlap. */
+typedef struct lw_batch {
+  int32_t seqs, tokens, max_new, max_kv;
+  const int32_t* q_start;    /* [seqs + 1] */
+  const int32_t* kv_len;     /* [seqs] */
+  const int32_t* page_table; /* [seqs][table_stride], the first table_pages of a row used */
+  int64_t table_stride;
+  int32_t table_pages;
+  int32_t reserved; /* 0 */
+  void* workspace;
+  int64_t workspace_bytes;
+} lw_batch;
+
+/* Bytes of workspace that attention of `heads` query heads over the batch needs, for any contents within max_new and
+ * max_kv. -1 on bad arguments. */
+long long lw_attn_workspace(const lw_kv_cache* cache, const lw_batch* batch, int heads);
+
+/* Appends the batch's new tokens to the cache and rotates on the way: with i a row's position and R_i the rotation of
+ * pairs (x, y) -> (x cos - y sin, y cos + x sin) by row i of cos / sin, cache k[i] = R_i k, cache v[i] = v and
+ * q_out = R_i q, each computed in fp32 and rounded once to the cache's type. q [tokens][heads][head_dim],
+ * k, v [tokens][kv_heads][head_dim] of x_type with row strides ldq, ldk, ldv (elements), q_out [tokens][heads][head_dim]
+ * of the cache's type with row stride ldo. Pointers are aligned to 16 bytes, strides multiples of 8. cos, sin: fp32
+ * [rope_rows][rot / 2], rope_rows >= max_kv, rot <= head_dim a multiple of 8: the first rot elements of a head are rotated, as
+ * pairs (j, j + rot / 2), or with neighbours = 1 as pairs (2 j, 2 j + 1); the others are copied. rot = 0: no rotation. q
+ * may be NULL (keys and values only). Rows of no sequence are left alone. Needs no workspace. Asynchronous on `stream`,
+ * allocates nothing, can be captured. Returns 0 or -1. */
+int lw_kv_append(const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, const void* k, const void* v,
+                 int x_type, long long ldq, long long ldk, long long ldv, const float* cos, const float* sin, int rot,
+                 int rope_rows, int neighbours, void* q_out, long long ldo, void* stream);
+
+/* Attention of the batch's new tokens over the cache, after lw_kv_append: out[t][h] = sum_j p_j v[j] / sum_j p_j over the
+ * positions j <= i that row t (position i) sees, p_j = exp(scale q[t][h] . k[j]), head h reading key-value head
+ * h / (heads / kv_heads); window > 0: only the last `window` of them (j > i - window). A row that sees nothing gives
+ * zeros; keys and values that a row does not see never reach it, whatever they hold. q [tokens][heads][head_dim] of
+ * the cache's type (row stride ldq), out of out_type (row stride ldo); alignment as lw_kv_append's. Scores, weights'
+ * sums and outputs are accumulated in fp32. lw_attn_decode is for max_new <= 16 (one new token per sequence, or a few
+ * that are verified together): the keys are split over the GPU and joined in order, the weights keep 22 bits or more.
+ * lw_attn_prompt takes any number; with a 16-bit out its weights are rounded to the cache's type, with LW_F32 they keep
+ * 22 bits or more. Both give the same bits on every call. Asynchronous on `stream`, allocate nothing, can be captured.
+ * Return 0 or -1. */
+int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, long long ldq, void* out,
+                   int out_type, long long ldo, float scale, int window, void* stream);
+int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, long long ldq, void* out,
+                   int out_type, long long ldo, float scale, int window, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

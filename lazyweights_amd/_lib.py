@@ -51,6 +51,11 @@ SIGNATURES = {
     "lw_set_prefill_gemm": (_i, [_i]),
     "lw_set_act8": (_i, [_i]),
     "lw_test_quant_x8": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp]),
+    # attention over a paged cache (lw_kv_cache and lw_batch by pointer)
+    "lw_attn_workspace": (_ll, [_vp, _vp, _i]),
+    "lw_kv_append": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _ll, _ll, _ll, _vp, _vp, _i, _i, _i, _vp, _ll, _vp]),
+    "lw_attn_decode": (_i, [_vp, _vp, _i, _vp, _ll, _vp, _i, _ll, _c.c_float, _i, _vp]),
+    "lw_attn_prompt": (_i, [_vp, _vp, _i, _vp, _ll, _vp, _i, _ll, _c.c_float, _i, _vp]),
 }
 
 _LIB = None

@@ -1,0 +1,178 @@
+"""Attention between a decoder layer's coded matrices, on torch tensors: a paged key-value cache, a batch of sequences over
+it, and the operators of include/lazyweights_amd.h that append to the cache and read it (lw_kv_append, lw_attn_decode,
+lw_attn_prompt).
+
+    cache = KvCache.empty(pages, kv_heads, page_size, head_dim)          # one per layer
+    batch = Batch(cache, heads, q_start, kv_len, page_table, max_new, max_kv)  # one for all layers
+    q16 = cache.append(batch, q, k, v, cos, sin)                         # q, k, v as the matrices give them, fp32
+    y = cache.attend_decode(batch, q16)                                  # or attend_prompt, for more than 16 new tokens
+
+The tensors of a batch (q_start, kv_len, page_table) are read on the GPU when a call runs: a program that writes the next
+step's lengths and pages into them keeps the batch, and can capture its calls, as long as max_new and max_kv bound them.
+Calls go to torch's current stream unless `stream` (a hipStream_t as an integer) is given. Bad arguments raise ValueError;
+a call that the library refuses raises RuntimeError with lw_last_error().
+"""
+import ctypes
+
+from ._lib import last_error, load_library
+
+F32, F16, BF16 = 0, 1, 2
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pages", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("type", ctypes.c_int32)]
+
+
+class _Batch(ctypes.Structure):
+    _fields_ = [("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_new", ctypes.c_int32),
+                ("max_kv", ctypes.c_int32), ("q_start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+                ("page_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_pages", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
+def _types():
+    import torch
+    return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+class Batch:
+    """`seqs` sequences whose new tokens are the rows of a call: q_start int32 [seqs + 1], kv_len int32 [seqs] (the lengths
+    with the new tokens), page_table int32 [seqs, pages], all on the cache's GPU. max_new and max_kv bound every
+    sequence's new tokens and length. A call's tensors may have more rows than q_start names; those are left alone. Holds
+    the workspace of attend_decode, so calls with one batch must not overlap."""
+
+    def __init__(self, cache, heads, q_start, kv_len, page_table, max_new, max_kv):
+        import torch
+        seqs = kv_len.shape[0]
+        if q_start.shape != (seqs + 1,) or kv_len.dim() != 1 or page_table.dim() != 2 or page_table.shape[0] != seqs:
+            raise ValueError("q_start [seqs + 1], kv_len [seqs] and page_table [seqs, pages] are wanted, not %s, %s, %s"
+                             % (tuple(q_start.shape), tuple(kv_len.shape), tuple(page_table.shape)))
+        for t in (q_start, kv_len, page_table):
+            if t.dtype != torch.int32 or t.device != cache.k.device:
+                raise ValueError("q_start, kv_len and page_table must be int32 tensors on the cache's device")
+            if t.numel() and t.stride(-1) != 1:
+                raise ValueError("q_start, kv_len and the rows of page_table must be contiguous")
+        self.heads, self.max_new, self.max_kv = int(heads), int(max_new), int(max_kv)
+        self.tensors = (q_start, kv_len, page_table)  # kept alive
+        self.c = _Batch(seqs, 0, self.max_new, self.max_kv, q_start.data_ptr(), kv_len.data_ptr(),
+                        page_table.data_ptr(), page_table.stride(0) if seqs > 1 else page_table.shape[1],
+                        page_table.shape[1], 0, None, 0)
+        self.ptr = ctypes.addressof(self.c)
+        size = cache.lib.lw_attn_workspace(cache.ptr, self.ptr, self.heads)
+        if size < 0:
+            raise ValueError(last_error())
+        self.workspace = torch.zeros(size, dtype=torch.uint8, device=cache.k.device)
+        self.c.workspace, self.c.workspace_bytes = self.workspace.data_ptr(), size
+
+
+class KvCache:
+    """Keys and values [pages, kv_heads, page_size, head_dim] of one layer, float16 or bfloat16 on the GPU, the caller's
+    tensors or views of them with head_dim contiguous (k and v alike in their strides)."""
+
+    def __init__(self, k, v):
+        types = _types()
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
+            raise ValueError("k and v must be [pages, kv_heads, page_size, head_dim], alike in type, device and strides")
+        if not k.is_cuda or types.get(k.dtype) not in (F16, BF16):
+            raise ValueError("k and v must be float16 or bfloat16 tensors on the GPU")
+        if k.stride(3) != 1:
+            raise ValueError("the elements of a head must be contiguous")
+        self.lib, self.k, self.v = load_library(), k, v
+        self.kv_heads, self.head_dim = k.shape[1], k.shape[3]
+        self.types = types
+        self.c = _Cache(k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), k.stride(2), k.shape[2],
+                        k.shape[1], k.shape[3], types[k.dtype])
+        self.ptr = ctypes.addressof(self.c)
+
+    @classmethod
+    def empty(cls, pages, kv_heads, page_size, head_dim, dtype=None, device="cuda"):
+        """A new cache of float16 (or `dtype`); its contents are whatever the memory held."""
+        import torch
+        k, v = (torch.empty((pages, kv_heads, page_size, head_dim), dtype=dtype or torch.float16, device=device)
+                for _ in range(2))
+        return cls(k, v)
+
+    def _rows(self, what, x, heads):
+        """Address and row stride of x [tokens, heads, head_dim] or [tokens, heads * head_dim]."""
+        shape, stride = x.shape, x.stride()
+        if len(shape) == 3:
+            ok = shape[1] == heads and shape[2] == self.head_dim and stride[2] == 1 and (
+                heads == 1 or stride[1] == self.head_dim)
+        else:
+            ok = len(shape) == 2 and shape[1] == heads * self.head_dim and stride[1] == 1
+        if not ok or x.device != self.k.device:
+            raise ValueError("%s: [tokens, %d, %d] (or the two last joined) with contiguous rows on the cache's device is "
+                             "wanted, not %s" % (what, heads, self.head_dim, tuple(shape)))
+        return x.data_ptr(), stride[0] if shape[0] > 1 else heads * self.head_dim
+
+    def _stream(self, stream):
+        if stream is not None:
+            return stream
+        import torch
+        return torch.cuda.current_stream(self.k.device).cuda_stream
+
+    def append(self, batch, q, k, v, cos=None, sin=None, q_out=None, neighbours=False, stream=None):
+        """Appends the rows k, v [tokens, kv_heads, head_dim] of the batch's new tokens, k rotated by its position, and
+        returns q [tokens, heads, head_dim], rotated alike, in the cache's type (q may be None: keys and values only).
+        q, k and v have one type (float32, float16 or bfloat16); rows may be views into a joined projection. cos, sin
+        float32 [positions, rot / 2] rotate the first rot elements of a head in pairs (j, j + rot / 2), or (2 j, 2 j + 1)
+        with `neighbours`; without them nothing is rotated."""
+        import torch
+        heads, n = batch.heads, k.shape[0]
+        kind = self.types.get(k.dtype)
+        if kind is None or v.dtype != k.dtype or v.shape[0] != n or (q is not None and (q.dtype != k.dtype or q.shape[0] != n)):
+            raise ValueError("q, k and v must have one of the types float32, float16, bfloat16 and the same number of rows")
+        kp, ldk = self._rows("k", k, self.kv_heads)
+        vp, ldv = self._rows("v", v, self.kv_heads)
+        qp, ldq, op, ldo = None, 0, None, 0
+        if q is not None:
+            qp, ldq = self._rows("q", q, heads)
+            if q_out is None:
+                q_out = torch.empty((n, heads, self.head_dim), dtype=self.k.dtype, device=self.k.device)
+            elif q_out.dtype != self.k.dtype or q_out.shape[0] != n:
+                raise ValueError("q_out must have the cache's type and q's rows")
+            op, ldo = self._rows("q_out", q_out, heads)
+        cp, sp, rot, rows = None, None, 0, 0
+        if cos is not None or sin is not None:
+            if (cos is None or sin is None or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2
+                    or cos.shape != sin.shape or cos.device != self.k.device or sin.device != self.k.device
+                    or not cos.is_contiguous() or not sin.is_contiguous()):
+                raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
+            cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
+        batch.c.tokens = n
+        if self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
+                                 1 if neighbours else 0, op, ldo, self._stream(stream)) != 0:
+            raise RuntimeError(last_error())
+        return q_out
+
+    def _attend(self, call, batch, q, out, scale, window, stream):
+        import torch
+        heads = batch.heads
+        if q.dtype != self.k.dtype:
+            raise ValueError("q must have the cache's type")
+        qp, ldq = self._rows("q", q, heads)
+        if out is None:
+            out = torch.empty(q.shape, dtype=self.k.dtype, device=self.k.device)
+        kind = self.types.get(out.dtype)
+        if kind is None or out.shape[0] != q.shape[0]:
+            raise ValueError("out must be float32, float16 or bfloat16, with q's rows")
+        op, ldo = self._rows("out", out, heads)
+        batch.c.tokens = q.shape[0]
+        if call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
+                window, self._stream(stream)) != 0:
+            raise RuntimeError(last_error())
+        return out
+
+    def attend_decode(self, batch, q, out=None, scale=None, window=0, stream=None):
+        """Attention of at most 16 new tokens per sequence over the cache, q [tokens, heads, head_dim] as append gives it:
+        every row sees the positions up to its own (the last `window` of them if window > 0), weights
+        softmax(scale q . k), scale 1 / sqrt(head_dim) by default. Returns out (q's type by default; float32, float16 and
+        bfloat16 can be given). A row that sees nothing gives zeros."""
+        return self._attend(self.lib.lw_attn_decode, batch, q, out, scale, window, stream)
+
+    def attend_prompt(self, batch, q, out=None, scale=None, window=0, stream=None):
+        """attend_decode for any number of new tokens: whole prompts, or chunks of them after what is in the cache."""
+        return self._attend(self.lib.lw_attn_prompt, batch, q, out, scale, window, stream)

@@ -1,0 +1,64 @@
+// Attention over a paged key-value cache: arguments of the kernels and their launchers (host interface of
+// lw_attention.hip; the C-ABI in lw_attn_api.cpp checks what a caller gives and fills these).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+#include <string>
+
+namespace lw {
+
+// Sets lw_last_error() of the calling thread.
+void set_error(const std::string& m);
+
+// The cache and the batch, as every kernel takes them. Key j of sequence s is row j & (2^page_shift - 1) of page
+// table[s * tstride + (j >> page_shift)]; a page outside [0, pages) holds no keys. The batch's rows are its new tokens:
+// those of sequence s are [q_start[s], q_start[s + 1]), its last ones, so row t has position kv_len[s] - q_start[s + 1] + t.
+struct KvView {
+  uint16_t *k, *v;
+  int64_t pstride, hstride, rstride;  // elements from a page, a head, a row to the next
+  const int32_t *q_start, *kv_len, *table;
+  int64_t tstride;
+  uint32_t pages;
+  int page_shift, table_pages;
+  int kv_heads, seqs, tokens;
+};
+
+struct AppendArgs {
+  KvView c;
+  const void *q, *k, *v;
+  int64_t ldq, ldk, ldv, ldo;
+  uint16_t* q_out;
+  const float *cos, *sin;  // [rope_rows][rot / 2]
+  int heads, rot, rope_rows, neighbours;
+};
+
+struct AttnArgs {
+  KvView c;
+  const uint16_t* q;
+  void* out;
+  int64_t ldq, ldo;
+  int out_type;
+  int heads, group;  // group = heads / kv_heads
+  float scale;       // of the scores, times log2(e): weights are powers of two
+  int window;        // > 0: a row sees its last `window` positions
+  // the decode kernel's split of the keys
+  float* part;
+  uint32_t* count;
+  int splits, chunk, row_blocks;
+};
+
+// How the decode kernel divides a batch: row_tiles tiles of 16 (token, head) rows per block, row_blocks of them, and the
+// keys in chunks of `chunk`, at most `splits`.
+struct DecodePlan {
+  int row_tiles, row_blocks, splits, chunk;
+  size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
+};
+DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);
+
+hipError_t launch_append(const AppendArgs& a, int head_dim, int type, int x_type, hipStream_t s);
+hipError_t launch_attn_decode(const AttnArgs& a, const DecodePlan& p, int head_dim, int type, hipStream_t s);
+hipError_t launch_attn_prompt(const AttnArgs& a, int head_dim, int type, hipStream_t s);
+
+}  // namespace lw

@@ -29,6 +29,7 @@
 #include <vector>
 
 #include "../../include/lazyweights_amd.h"
+#include "lw_attention.h"
 #include "lw_codec.h"
 #include "lw_format.h"
 #include "lw_kernels.h"
@@ -1624,6 +1625,10 @@ int copy_out(Model& M, uint8_t* out, const uint8_t* src, size_t n) {
 }  // namespace
 
 // ── C-ABI ────────────────────────────────────────────────────────────────────────────────────────────────
+
+namespace lw {
+void set_error(const std::string& m) { g_err = m; }
+}  // namespace lw
 
 extern "C" {
 
