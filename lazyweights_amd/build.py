@@ -32,7 +32,8 @@ SOURCES = [
     ("lw_kernels.hip", "hip"),
     ("lw_wide.hip", "hip"),
     ("lw_prefill.hip", "hip"),
-    ("lw_attention.hip", "hip"),
+    ("lw_attn_decode.hip", "hip"),
+    ("lw_attn_prompt.hip", "hip"),
     ("lw_runtime.cpp", "hiphost"),
     ("lw_attn_api.cpp", "hiphost"),
     ("lw_codec.cpp", "cxx"),

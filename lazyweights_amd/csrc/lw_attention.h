@@ -1,5 +1,5 @@
 // Attention over a paged key-value cache: arguments of the kernels and their launchers (host interface of
-// lw_attention.hip; the C-ABI in lw_attn_api.cpp checks what a caller gives and fills these).
+// lw_attn_decode.hip and lw_attn_prompt.hip; the C-ABI in lw_attn_api.cpp checks what a caller gives and fills these).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -43,16 +43,16 @@ struct AttnArgs {
   int heads, group;  // group = heads / kv_heads
   float scale;       // of the scores, times log2(e): weights are powers of two
   int window;        // > 0: a row sees its last `window` positions
-  // the decode kernel's split of the keys
+  // the decode kernel's workspace and division (DecodePlan)
   float* part;
   uint32_t* count;
-  int splits, chunk, row_blocks;
+  int row_blocks, min_run;
 };
 
-// How the decode kernel divides a batch: row_tiles tiles of 16 (token, head) rows per block, row_blocks of them, and the
-// keys in chunks of `chunk`, at most `splits`.
+// How the decode kernel divides a batch: row_tiles tiles of 16 (token, head) rows per item, row_blocks items for a
+// sequence's key-value head, blocks of the launch, and the least tiles of 32 keys that one takes.
 struct DecodePlan {
-  int row_tiles, row_blocks, splits, chunk;
+  int row_tiles, row_blocks, blocks, min_run;
   size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
 };
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);

@@ -95,7 +95,7 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   a.window = (int)std::min<long long>(window, kMostRows);
   a.part = nullptr;
   a.count = nullptr;
-  a.splits = a.chunk = a.row_blocks = 0;
+  a.row_blocks = a.min_run = 0;
   return 0;
 }
 
@@ -161,15 +161,13 @@ int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
   if (batch->max_new > 16) return refuse(fn, "max_new is more than 16 (lw_attn_prompt takes any number)");
   const lw::DecodePlan p = lw::decode_plan(batch->seqs, cache->kv_heads, a.group, cache->head_dim, batch->max_new,
                                            batch->max_kv);
-  if ((long long)cache->kv_heads * p.row_blocks > 65535) return refuse(fn, "more heads than a launch can take");
   if (!batch->workspace || (reinterpret_cast<uintptr_t>(batch->workspace) & 15) ||
       batch->workspace_bytes < (long long)(p.count_bytes + p.part_bytes))
     return refuse(fn, "needs a workspace of " + std::to_string(p.count_bytes + p.part_bytes) + " bytes, aligned to 16");
   a.count = static_cast<uint32_t*>(batch->workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(batch->workspace) + p.count_bytes);
-  a.splits = p.splits;
-  a.chunk = p.chunk;
   a.row_blocks = p.row_blocks;
+  a.min_run = p.min_run;
   return launched(fn, lw::launch_attn_decode(a, p, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
 }
 
