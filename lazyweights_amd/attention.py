@@ -14,6 +14,11 @@ a call that the library refuses raises RuntimeError with lw_last_error().
 """
 import ctypes
 
+try:
+    import torch
+except ImportError:  # (bundles and the host entry points need none)
+    torch = None
+
 from ._lib import last_error, load_library
 
 F32, F16, BF16 = 0, 1, 2
@@ -34,8 +39,13 @@ class _Batch(ctypes.Structure):
 
 
 def _types():
-    import torch
     return {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+
+
+def _current_stream():
+    """A function: device index -> torch's current stream there, as an integer."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a tenth of the public call's 2 us
+    return raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class Batch:
@@ -45,7 +55,6 @@ class Batch:
     the workspace of attend_decode, so calls with one batch must not overlap."""
 
     def __init__(self, cache, heads, q_start, kv_len, page_table, max_new, max_kv):
-        import torch
         seqs = kv_len.shape[0]
         if q_start.shape != (seqs + 1,) or kv_len.dim() != 1 or page_table.dim() != 2 or page_table.shape[0] != seqs:
             raise ValueError("q_start [seqs + 1], kv_len [seqs] and page_table [seqs, pages] are wanted, not %s, %s, %s"
@@ -82,7 +91,8 @@ class KvCache:
             raise ValueError("the elements of a head must be contiguous")
         self.lib, self.k, self.v = load_library(), k, v
         self.kv_heads, self.head_dim = k.shape[1], k.shape[3]
-        self.types = types
+        self.types, self.index = types, k.get_device()
+        self._current = _current_stream()
         self.c = _Cache(k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), k.stride(2), k.shape[2],
                         k.shape[1], k.shape[3], types[k.dtype])
         self.ptr = ctypes.addressof(self.c)
@@ -90,29 +100,21 @@ class KvCache:
     @classmethod
     def empty(cls, pages, kv_heads, page_size, head_dim, dtype=None, device="cuda"):
         """A new cache of float16 (or `dtype`); its contents are whatever the memory held."""
-        import torch
         k, v = (torch.empty((pages, kv_heads, page_size, head_dim), dtype=dtype or torch.float16, device=device)
                 for _ in range(2))
         return cls(k, v)
 
     def _rows(self, what, x, heads):
         """Address and row stride of x [tokens, heads, head_dim] or [tokens, heads * head_dim]."""
-        shape, stride = x.shape, x.stride()
+        shape, stride, dim = x.shape, x.stride(), self.head_dim
         if len(shape) == 3:
-            ok = shape[1] == heads and shape[2] == self.head_dim and stride[2] == 1 and (
-                heads == 1 or stride[1] == self.head_dim)
+            ok = shape[1] == heads and shape[2] == dim and stride[2] == 1 and (heads == 1 or stride[1] == dim)
         else:
-            ok = len(shape) == 2 and shape[1] == heads * self.head_dim and stride[1] == 1
-        if not ok or x.device != self.k.device:
+            ok = len(shape) == 2 and shape[1] == heads * dim and stride[1] == 1
+        if not ok or x.get_device() != self.index:
             raise ValueError("%s: [tokens, %d, %d] (or the two last joined) with contiguous rows on the cache's device is "
-                             "wanted, not %s" % (what, heads, self.head_dim, tuple(shape)))
-        return x.data_ptr(), stride[0] if shape[0] > 1 else heads * self.head_dim
-
-    def _stream(self, stream):
-        if stream is not None:
-            return stream
-        import torch
-        return torch.cuda.current_stream(self.k.device).cuda_stream
+                             "wanted, not %s" % (what, heads, dim, tuple(shape)))
+        return x.data_ptr(), stride[0] if shape[0] > 1 else heads * dim
 
     def append(self, batch, q, k, v, cos=None, sin=None, q_out=None, neighbours=False, stream=None):
         """Appends the rows k, v [tokens, kv_heads, head_dim] of the batch's new tokens, k rotated by its position, and
@@ -120,7 +122,6 @@ class KvCache:
         q, k and v have one type (float32, float16 or bfloat16); rows may be views into a joined projection. cos, sin
         float32 [positions, rot / 2] rotate the first rot elements of a head in pairs (j, j + rot / 2), or (2 j, 2 j + 1)
         with `neighbours`; without them nothing is rotated."""
-        import torch
         heads, n = batch.heads, k.shape[0]
         kind = self.types.get(k.dtype)
         if kind is None or v.dtype != k.dtype or v.shape[0] != n or (q is not None and (q.dtype != k.dtype or q.shape[0] != n)):
@@ -138,18 +139,17 @@ class KvCache:
         cp, sp, rot, rows = None, None, 0, 0
         if cos is not None or sin is not None:
             if (cos is None or sin is None or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2
-                    or cos.shape != sin.shape or cos.device != self.k.device or sin.device != self.k.device
+                    or cos.shape != sin.shape or cos.get_device() != self.index or sin.get_device() != self.index
                     or not cos.is_contiguous() or not sin.is_contiguous()):
                 raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
             cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
         batch.c.tokens = n
         if self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
-                                 1 if neighbours else 0, op, ldo, self._stream(stream)) != 0:
+                                 1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream) != 0:
             raise RuntimeError(last_error())
         return q_out
 
     def _attend(self, call, batch, q, out, scale, window, stream):
-        import torch
         heads = batch.heads
         if q.dtype != self.k.dtype:
             raise ValueError("q must have the cache's type")
@@ -162,7 +162,7 @@ class KvCache:
         op, ldo = self._rows("out", out, heads)
         batch.c.tokens = q.shape[0]
         if call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
-                window, self._stream(stream)) != 0:
+                window, self._current(self.index) if stream is None else stream) != 0:
             raise RuntimeError(last_error())
         return out
 

@@ -41,7 +41,8 @@ struct AttnArgs {
   int64_t ldq, ldo;
   int out_type;
   int heads, group;  // group = heads / kv_heads
-  float scale;       // of the scores, times log2(e): weights are powers of two
+  float scale;       // of the scores, times log2(e) (weights are powers of two), positive
+  uint32_t q_flip;   // the sign bits of two elements where the caller's scale is negative: q is negated instead
   int window;        // > 0: a row sees its last `window` positions
   // the decode kernel's workspace and division (DecodePlan)
   float* part;

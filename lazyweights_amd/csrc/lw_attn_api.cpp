@@ -91,7 +91,10 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   a.out_type = out_type;
   a.heads = heads;
   a.group = heads / cache->kv_heads;
-  a.scale = scale * 1.4426950408889634f;
+  // (0 stands for the least normal number and more: products with it are 0 to any purpose, and -infinity, which marks what a
+  // row does not see, stays what it is)
+  a.scale = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-37f);
+  a.q_flip = scale < 0 ? 0x80008000u : 0;
   a.window = (int)std::min<long long>(window, kMostRows);
   a.part = nullptr;
   a.count = nullptr;

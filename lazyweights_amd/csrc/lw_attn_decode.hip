@@ -111,7 +111,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
     pos[t] = r < R ? past + r / a.group : -1;
     const uint16_t* q = a.q + (int64_t)(sq.row0 + r / a.group) * a.ldq + (int64_t)(kvh * a.group + r % a.group) * D + 8 * g;
 #pragma unroll
-    for (int i = 0; i < C; ++i) qf[t][i] = r < R ? *reinterpret_cast<const u32x4*>(q + 32 * i) : (u32x4)0;
+    for (int i = 0; i < C; ++i) qf[t][i] = r < R ? *reinterpret_cast<const u32x4*>(q + 32 * i) ^ a.q_flip : (u32x4)0;
   }
   const int32_t* table = c.table + s * c.tstride;
   const uint16_t* kb = c.k + kvh * c.hstride + 8 * g;

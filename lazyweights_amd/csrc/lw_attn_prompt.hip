@@ -12,19 +12,20 @@ namespace {
 // the score product's operand reads (32 keys of a chunk) and the transposed reads of V (4 keys of 4 chunks) are both free
 // of bank conflicts. The next tile is loaded into registers while one is worked on.
 template <int D, bool BF, int NP>
-__global__ __launch_bounds__(256) void k_attn_prompt(const AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void k_attn_prompt(const AttnArgs a) {
   constexpr int C = D / 32, ROWS = 128, BLK = D * 16;  // BLK: elements of a 16-key block
   __shared__ __align__(16) uint16_t kl[2][4 * BLK], vl[2][4 * BLK];
   __shared__ uint16_t seen_l[2][4];
+  __shared__ float care[4][16 * 32];  // weights of 16 keys x 32 rows of each wave, in the second pass
   __shared__ int any_bad;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n = lane & 31, g = lane >> 5;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
   const KvView& c = a.c;
   const int kvh = blockIdx.x % c.kv_heads, tile = (int)(gridDim.x / c.kv_heads) - 1 - (int)(blockIdx.x / c.kv_heads);
   // sequence s owns tiles from q_start[s] group / ROWS + s on: at least as many as its rows take
   auto first_tile = [&](int i) {
     return (int)((int64_t)clampi(c.q_start[i], 0, c.tokens) * a.group / ROWS) + i;
   };
-  const int s = last_at_most(c.seqs, tile, first_tile);
+  const int s = __builtin_amdgcn_readfirstlane(last_at_most(c.seqs, tile, first_tile));
   const Seq sq = sequence(c, s);
   const int R = sq.rows * a.group, r0 = (tile - first_tile(s)) * ROWS;
   if (r0 < 0 || r0 >= R) return;
@@ -42,7 +43,8 @@ __global__ __launch_bounds__(256) void k_attn_prompt(const AttnArgs a) {
   u32x4 qf[2 * C];
 #pragma unroll
   for (int i = 0; i < 2 * C; ++i)
-    qf[i] = row < R ? *reinterpret_cast<const u32x4*>(a.q + (int64_t)(sq.row0 + tok) * a.ldq + (int64_t)head * D + 16 * i + 8 * g)
+    qf[i] = row < R ? *reinterpret_cast<const u32x4*>(a.q + (int64_t)(sq.row0 + tok) * a.ldq + (int64_t)head * D + 16 * i + 8 * g) ^
+                          a.q_flip
                     : (u32x4)0;
 
   // staging: wave w loads the 16 keys of block w, lane l row (l - 4 (l >> 4)) & 15, chunks 4 i + (l >> 4)
@@ -107,55 +109,58 @@ __global__ __launch_bounds__(256) void k_attn_prompt(const AttnArgs a) {
             sc[h] = mfma32<BF>(kf, qf[i], sc[h]);
           }
         }
-        const bool all = seen == ~0ull && full && t0 + 64 <= min(wlo + 1, hi) && (a.window <= 0 || t0 > whi - a.window);
-        float p[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) p[e] = sc[e >> 4][e & 15] * a.scale;
-        if (!all) {
-          const int first = a.window > 0 ? pos - a.window : -1;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int k = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + 4 * g + (e & 3), key = t0 + k;
-            if (!(key <= pos && key > first && key < hi && ((seen >> k) & 1))) p[e] = -INFINITY;
-          }
-        }
-        float mx = p[0];
-#pragma unroll
-        for (int e = 1; e < 32; ++e) mx = fmaxf(mx, p[e]);
-        mx = fmaxf(max32(mx), m);
-        const float base = mx == -INFINITY ? 0.f : mx, down = pow2(m - base);
-        m = mx;
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float v = pow2(p[e] - base);
-          sum += v;
-          if (CAREFUL && p[e] == -INFINITY) p[e] = -1.f;
-          else p[e] = v;
-        }
-        l = l * down + sum;
-#pragma unroll
-        for (int d = 0; d < C; ++d) o[d] *= down;
-        if (CAREFUL) {
+        if (!(seen == ~0ull && full && t0 + 64 <= min(wlo + 1, hi) && (a.window <= 0 || t0 > whi - a.window))) {
+          // bit k: this lane's row sees key t0 + k
+          const int end = min(min(pos + 1, hi) - t0, 64), begin = a.window > 0 ? max(pos - a.window + 1 - t0, 0) : 0;
+          uint64_t bits = end > begin && begin < 64 ? (~0ull >> (64 - end + begin)) << begin & seen : 0;
+          bits >>= 4 * g;
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            for (int kg = 0; kg < 2; ++kg) {
-              const float pk = __shfl(p[e], 32 * kg + n);
-              const int k = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + 4 * kg + (e & 3);
+            if (!((uint32_t)(bits >> (e & 16 ? 32 : 0)) & (1u << (8 * ((e >> 2) & 3) + (e & 3))))) sc[e >> 4][e & 15] = -INFINITY;
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
+        mx = max32(mx) * a.scale;
+        // weights are 2^(score - m); m follows the largest score only when that is far ahead of it (a weight is at most 2^8
+        // then: no range is lost), since moving it costs a product of every sum
+        if (__any(mx > m + 8.f)) {
+          const float up = fmaxf(m, mx), down = m == -INFINITY ? 0.f : pow2(m - up);
+          m = up;
+          l *= down;
+#pragma unroll
+          for (int d = 0; d < C; ++d) o[d] *= down;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float p[32], sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const float x = sc[e >> 4][e & 15], v = pow2(__builtin_fmaf(x, a.scale, -base));
+          sum += v;
+          p[e] = CAREFUL && x == -INFINITY ? -1.f : v;  // (-1: not seen)
+        }
+        l += sum;
+        if constexpr (CAREFUL) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) care[w][(8 * (e >> 2) + 4 * g + (e & 3)) * 32 + n] = p[8 * q + e];
+#pragma unroll 1
+            for (int k = 0; k < 16; ++k) {
+              const float pk = care[w][k * 32 + n];
 #pragma unroll
               for (int d = 0; d < C; ++d)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // dims 32 d + 8 j + 4 g + i: chunk 4 d + j
                   const int ch = 4 * d + j;
-                  const uint2 u = *reinterpret_cast<const uint2*>(
-                      &vl[b][(k >> 4) * BLK + ch * 128 + (((k & 15) + 4 * ch) & 15) * 8 + 4 * g]);
+                  const uint2 u = *reinterpret_cast<const uint2*>(&vl[b][q * BLK + ch * 128 + ((k + 4 * ch) & 15) * 8 + 4 * g]);
                   const f4v v = {wide<BF>((uint16_t)u.x), wide<BF>((uint16_t)(u.x >> 16)), wide<BF>((uint16_t)u.y),
                                  wide<BF>((uint16_t)(u.y >> 16))};
-                  if (!(pk < 0.f))
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[d][4 * j + i] += pk * v[i];
+                  for (int i = 0; i < 4; ++i) o[d][4 * j + i] = pk < 0.f ? o[d][4 * j + i] : o[d][4 * j + i] + pk * v[i];
                 }
             }
+          }
         } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {  // 16 keys: 16 q + 4 g + i and 16 q + 8 + 4 g + i
