@@ -495,3 +495,34 @@ def test_python_refusals(gpu, lib):
         cache.attend_decode(many, q)
     cache.attend_prompt(many, q)
     torch.cuda.synchronize()
+
+
+MANY = [
+    # dim, page, type, out, window: 512 rows of 512 heads, enough blocks for the form with 8 waves
+    (64, 16, "float16", "float16", 0),
+    (96, 8, "bfloat16", "float32", 0),
+    (128, 64, "float16", "float32", 70),
+    (128, 16, "bfloat16", "bfloat16", 0),
+    (64, 32, "bfloat16", "float32", 33),
+    (96, 16, "float16", "float16", 200),
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=str)
+def test_prompt_of_many_rows(gpu, lib, case):
+    """Rows that see 1 to 6 key tiles in blocks of 256, a hidden NaN among the values, a part of the rows of a block."""
+    import torch
+    dim, page, dtype, out, window = case
+    dtype, out = getattr(torch, dtype), getattr(torch, out)
+    layout, lengths = (512, 512, dim), [(300, 0), (0, 5), (150, 200), (1, 0), (61, 64)]
+    k, v, table, q_start, kv_len, q = make(torch, layout, page, dtype, lengths, 27)
+    cache, batch = build(torch, layout, k, v, table, q_start, kv_len, 300, 350)
+    ref = reference(torch, k, v, table, lengths, q, window, dim ** -0.5)
+    y = cache.attend_prompt(batch, q, out=torch.full(q.shape, float("nan"), dtype=out, device="cuda"), window=window)
+    check(torch, y, ref, dtype, True)
+    v[int(table[0, 250 // page]), :, 250 % page] = float("nan")  # rows 250 .. 299 of the first sequence see it
+    y = cache.attend_prompt(batch, q, out=torch.empty_like(q, dtype=out), window=window)
+    seen = torch.zeros(512, dtype=torch.bool, device="cuda")
+    seen[250:min(300, 250 + window) if window else 300] = True
+    assert torch.isnan(y[seen]).all()
+    check(torch, y[~seen], [t[~seen] for t in ref], dtype, True)
