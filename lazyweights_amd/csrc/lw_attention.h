@@ -34,6 +34,19 @@ struct AppendArgs {
   int heads, rot, rope_rows, neighbours;
 };
 
+// x / d for 0 <= x < 2^31 as a product and a shift: the product of x and ceil(2^(31 + k) / d), 2^k the power of two at or
+// above d, is less than 2^31 too large
+struct Divisor {
+  uint64_t mul;
+  int shift;
+  __host__ __device__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * mul) >> shift); }
+};
+inline Divisor divisor(int d) {
+  int k = 0;
+  while ((1u << k) < (uint32_t)d) ++k;
+  return {(((uint64_t)1 << (31 + k)) + d - 1) / d, 31 + k};
+}
+
 struct AttnArgs {
   KvView c;
   const uint16_t* q;
@@ -41,19 +54,21 @@ struct AttnArgs {
   int64_t ldq, ldo;
   int out_type;
   int heads, group;  // group = heads / kv_heads
+  Divisor by_group;
   float scale;       // of the scores, times log2(e) (weights are powers of two), positive
   uint32_t q_flip;   // the sign bits of two elements where the caller's scale is negative: q is negated instead
   int window;        // > 0: a row sees its last `window` positions
   // the decode kernel's workspace and division (DecodePlan)
   float* part;
   uint32_t* count;
-  int row_blocks, min_run;
+  int row_blocks, blocks_log2, most_keys;
 };
 
 // How the decode kernel divides a batch: row_tiles tiles of 16 (token, head) rows per item, row_blocks items for a
-// sequence's key-value head, blocks of the launch, and the least tiles of 32 keys that one takes.
+// sequence's key-value head, and a power of two of blocks. The list of all items' tiles of 32 keys is counted in 32 bits:
+// most_keys is the most of a sequence that keeps it there (2^31 tiles in all).
 struct DecodePlan {
-  int row_tiles, row_blocks, blocks, min_run;
+  int row_tiles, row_blocks, blocks_log2, most_keys;
   size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
 };
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);

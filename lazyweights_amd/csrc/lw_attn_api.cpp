@@ -91,6 +91,7 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   a.out_type = out_type;
   a.heads = heads;
   a.group = heads / cache->kv_heads;
+  a.by_group = lw::divisor(a.group);
   // (0 stands for the least normal number and more: products with it are 0 to any purpose, and -infinity, which marks what a
   // row does not see, stays what it is)
   a.scale = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-37f);
@@ -98,7 +99,7 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   a.window = (int)std::min<long long>(window, kMostRows);
   a.part = nullptr;
   a.count = nullptr;
-  a.row_blocks = a.min_run = 0;
+  a.row_blocks = a.blocks_log2 = a.most_keys = 0;
   return 0;
 }
 
@@ -164,13 +165,15 @@ int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
   if (batch->max_new > 16) return refuse(fn, "max_new is more than 16 (lw_attn_prompt takes any number)");
   const lw::DecodePlan p = lw::decode_plan(batch->seqs, cache->kv_heads, a.group, cache->head_dim, batch->max_new,
                                            batch->max_kv);
+  if (p.most_keys < batch->max_kv) return refuse(fn, "more sequences, heads and positions than a launch can take");
   if (!batch->workspace || (reinterpret_cast<uintptr_t>(batch->workspace) & 15) ||
       batch->workspace_bytes < (long long)(p.count_bytes + p.part_bytes))
     return refuse(fn, "needs a workspace of " + std::to_string(p.count_bytes + p.part_bytes) + " bytes, aligned to 16");
   a.count = static_cast<uint32_t*>(batch->workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(batch->workspace) + p.count_bytes);
   a.row_blocks = p.row_blocks;
-  a.min_run = p.min_run;
+  a.blocks_log2 = p.blocks_log2;
+  a.most_keys = p.most_keys;
   return launched(fn, lw::launch_attn_decode(a, p, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
 }
 

@@ -80,38 +80,30 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
 
 constexpr int NW = 4;  // waves of a block
 
-// x, known to be the same in every lane
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  return (int64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
-         (int64_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
-}
-// x / y of numbers that are not negative, in 32 bits where both fit
-__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
-  return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
-}
-
-// Tiles [t_from, t_to) of the item (s, kvh, rb), whose keys start at `lo`; blocks b0 .. b1 of the launch have a part of it.
+// Tiles [t_from, t_to) of the item (s, kvh, rb), whose keys start at `lo` and whose T tiles are the list's from item0 on; a block
+// has `run` tiles of the list.
 template <int D, bool BF, int RT>
 __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, float* ml, float* pcare, int* last_block, int s, const Seq& sq,
-                                            int kvh, int rb, int lo, int t_from, int t_to, int b0, int b1, int lane, int w,
-                                            int n, int g) {
+                                            int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0, int T,
+                                            uint32_t run, int lane, int w, int n, int g) {
   constexpr int C = D / 32, DT = D / 16, NP = BF ? 3 : 2;
   const KvView& c = a.c;
+  const Divisor by_group = a.by_group;
   const int R = sq.rows * a.group, r0 = rb * RT * 16;
   const int past = sq.len - sq.rows;  // row r has position past + r / group
-  const int rn = max(min(r0 + RT * 16, R) - 1, r0), pos_lo = past + r0 / a.group, pos_hi = past + rn / a.group;
+  const int rn = max(min(r0 + RT * 16, R) - 1, r0), pos_lo = past + by_group(r0), pos_hi = past + by_group(rn);
   const int k0 = lo + 32 * t_from, k1 = min(lo + 32 * t_to, sq.len), tiles = k1 > k0 && r0 < R ? t_to - t_from : 0;
-  const int active = b1 - b0 + 1;
 
+  const u32x4 flip = (u32x4)(uint32_t)__builtin_amdgcn_readfirstlane(a.q_flip);
   int pos[RT];
   u32x4 qf[RT][C];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    const int r = r0 + 16 * t + n;
-    pos[t] = r < R ? past + r / a.group : -1;
-    const uint16_t* q = a.q + (int64_t)(sq.row0 + r / a.group) * a.ldq + (int64_t)(kvh * a.group + r % a.group) * D + 8 * g;
+    const int r = r0 + 16 * t + n, tok = by_group(r);
+    pos[t] = r < R ? past + tok : 1 << 30;  // (past the last row: whatever, nothing is written)
+    const uint16_t* q = a.q + (int64_t)(sq.row0 + tok) * a.ldq + (int64_t)(kvh * a.group + r - tok * a.group) * D + 8 * g;
 #pragma unroll
-    for (int i = 0; i < C; ++i) qf[t][i] = r < R ? *reinterpret_cast<const u32x4*>(q + 32 * i) ^ a.q_flip : (u32x4)0;
+    for (int i = 0; i < C; ++i) qf[t][i] = r < R ? *reinterpret_cast<const u32x4*>(q + 32 * i) ^ flip : (u32x4)0;
   }
   const int32_t* table = c.table + s * c.tstride;
   const uint16_t* kb = c.k + kvh * c.hstride + 8 * g;
@@ -179,7 +171,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
         ask(t + NW);
         ask_page(min(t + 2 * NW, tiles - 1));
       }
-      const bool all = (seen[0] & seen[1]) == 0xFFFFu && t0 + 32 <= min(pos_lo + 1, k1) && r0 + RT * 16 <= R &&
+      const bool all = (seen[0] & seen[1]) == 0xFFFFu && t0 + 32 <= min(pos_lo + 1, k1) &&
                        (a.window <= 0 || t0 > pos_hi - a.window);
       u32x4 part[RT][NP];
       float p[RT][8];
@@ -268,7 +260,8 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
   // adds those of row x & 15, dims 4 (x >> 4) .. (and 64 on), in the waves' order.
   constexpr int RW = 16 * RT, TH = 64 * NW, Q = (4 * D + TH - 1) / TH;  // Q: groups of 4 dims per thread
   const int64_t item = ((int64_t)s * a.row_blocks + rb) * c.kv_heads + kvh;
-  // a block has two slots for its parts of items [RW] (m, l), [RW][D]: 2 b of one that began in an earlier run, 2 b + 1
+  const int b0 = (int)(item0 / run), b1 = (int)((item0 + T - 1) / run), active = b1 - b0 + 1;
+  // a block has two slots for its parts of items, [RW] (m, l), [RW][D]: 2 b for one that began in an earlier run, and 2 b + 1
   constexpr int SLOT = RW * (D + 2);
   auto slot = [&](int b) { return a.part + (int64_t)(2 * b + (b == b0)) * SLOT; };
 #pragma unroll
@@ -282,9 +275,10 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
   __syncthreads();
   float* ob = reinterpret_cast<float*>(smem);  // [NW waves][D / 4][16 rows][4]
   const int n2 = threadIdx.x & 15, q2 = threadIdx.x >> 4;
-  float* mine = slot(blockIdx.x);
+  float* my_slot = slot(blockIdx.x);
   auto out_at = [&](int row, int dim) {
-    return (int64_t)(sq.row0 + row / a.group) * a.ldo + (int64_t)(kvh * a.group + row % a.group) * D + dim;
+    const int tok = by_group(row);
+    return (int64_t)(sq.row0 + tok) * a.ldo + (int64_t)(kvh * a.group + row - tok * a.group) * D + dim;
   };
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
@@ -308,7 +302,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 #pragma unroll
     for (int i = 0; i < NW; ++i) sum += ml[(i * RW + lr) * 2 + 1] * pow2(ml[(i * RW + lr) * 2] - base);
     if (row < R) {
-      if (active > 1 && q2 == 0) put2(mine + lr * 2, mx, sum);
+      if (active > 1 && q2 == 0) put2(my_slot + lr * 2, mx, sum);
 #pragma unroll
       for (int k = 0; k < Q; ++k) {
         const int dq = q2 + TH / 16 * k;
@@ -317,7 +311,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 #pragma unroll
           for (int i = 1; i < NW; ++i) v += *reinterpret_cast<const f4v*>(ob + ((i * (D / 4) + dq) * 16 + n2) * 4);
           if (active > 1) {
-            float* p = mine + 2 * RW + lr * D + 4 * dq;
+            float* p = my_slot + 2 * RW + lr * D + 4 * dq;
             put2(p, v[0], v[1]);
             put2(p + 2, v[2], v[3]);
           } else {
@@ -378,11 +372,11 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
         }
     }
     if (groups > 1) {
-      float* mine = ob + threadIdx.x * 6;
-      mine[0] = mx;
-      mine[1] = sum;
+      float* z = ob + threadIdx.x * 6;
+      z[0] = mx;
+      z[1] = sum;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine[2 + i] = acc[i];
+      for (int i = 0; i < 4; ++i) z[2 + i] = acc[i];
       __syncthreads();
       if (cg == 0) {
         float top = mx;
@@ -404,74 +398,105 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 }
 
 // Work is a list of items (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as many tiles of 32
-// keys as the sequence's rows see together; the launch's blocks take equal runs of the list's tiles, whatever the lengths
-// (the prefix sums over the sequences are formed by every wave for itself). Within a run, a block's waves take the tiles of
-// an item in turn, each on its own (no barrier in the loop), and join at the item's end. An item that lies in several runs
-// is joined, in their order, by the block that ends last.
+// keys as the sequence's rows see together; the launch's blocks take equal runs of the list's tiles, whatever the lengths.
+// Within a run, a block's waves take the tiles of an item in turn, each on its own (no barrier in the loop), and join at
+// the item's end. An item that lies in several runs is joined, in their order, by the block that ends last.
 template <int D, bool BF, int RT>
 __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void k_attn_decode(const AttnArgs a) {
-  constexpr int C = D / 32, DT = D / 16, NP = BF ? 3 : 2;
   __shared__ __align__(16) uint8_t smem[NW * 32 * D * 2];  // V tiles of the waves; after the loop their sums
   __shared__ float ml[NW * 16 * RT * 2];
   __shared__ float pcare[NW * 32 * 16];
+  __shared__ uint32_t csum[1024];  // tiles of the sequences up to each 64th
   __shared__ int last_block;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   const KvView& c = a.c;
-  const int H = c.kv_heads * a.row_blocks;
+  const int seqs = c.seqs, kv_heads = c.kv_heads, H = kv_heads * a.row_blocks, chunks = (seqs + 63) >> 6;
   // tiles of each of a sequence's items: those of the keys [lo, len) that its rows see; one where they see none, to write
   // the zeros
   auto first_key = [&](const Seq& q) { return a.window > 0 ? max(0, q.len - q.rows - a.window + 1) & ~31 : 0; };
   auto tiles_of = [&](const Seq& q) { return q.rows ? max((q.len - first_key(q) + 31) >> 5, 1) : 0; };
-  int64_t total = 0;
-  for (int i = 0; i < c.seqs; i += 64) {
-    int64_t t = i + lane < c.seqs ? tiles_of(sequence(c, i + lane)) : 0;
-    for (int d = 1; d < min(64, c.seqs); d *= 2) t += __shfl_xor(t, d);
-    total += uniform(t);
-  }
-  total *= H;
-  const int64_t run = max(quotient(total + gridDim.x - 1, gridDim.x), (int64_t)a.min_run), from = run * blockIdx.x;
-  const int64_t to = min(from + run, total);
-  if (from >= to) return;
-  // the sequence that holds tile `from`, and the list's tiles before it
-  int s = 0;
-  int64_t before = 0;
-  for (int i = 0; i < c.seqs; i += 64) {
-    int64_t t = i + lane < c.seqs ? (int64_t)tiles_of(sequence(c, i + lane)) * H : 0;
-    const int64_t own = t;
-    for (int d = 1; d < min(64, c.seqs); d *= 2) {
-      const int64_t o = __shfl_up(t, d);
-      if (lane >= d) t += o;
+  // the sequences are held 64 at a time, one per lane, with their tiles and those up to theirs
+  Seq mine;
+  uint32_t own, upto;
+  int held;
+  auto hold = [&](int chunk) __attribute__((always_inline)) {
+    held = chunk;
+    mine = {0, 0, 0};
+    if (64 * chunk + lane < seqs) {
+      mine = sequence(c, 64 * chunk + lane);
+      mine.len = min(mine.len, a.most_keys);
     }
-    const uint64_t past = __ballot(before + t > from);  // lanes whose sequences end after it
-    if (past) {
-      const int j = __ffsll((unsigned long long)past) - 1;
-      s = i + j;
-      before += __shfl(t - own, j);
-      break;
+    upto = own = tiles_of(mine) * H;
+    for (int d = 1; d < min(64, seqs); d *= 2) {
+      const uint32_t o = __shfl_up(upto, d);
+      if (lane >= d) upto += o;
     }
-    before += __shfl(t, 63);  // (every lane's)
+  };
+  auto held_seq = [&](int j) __attribute__((always_inline)) {
+    return Seq{__builtin_amdgcn_readlane(mine.row0, j), __builtin_amdgcn_readlane(mine.rows, j),
+               __builtin_amdgcn_readlane(mine.len, j)};
+  };
+  uint32_t total;
+  if (chunks == 1) {
+    hold(0);
+    total = __builtin_amdgcn_readlane(upto, min(seqs, 64) - 1);
+  } else {
+    for (int i = w; i < chunks; i += NW) {
+      hold(i);
+      if (lane == 63) csum[i] = upto;
+    }
+    __syncthreads();
+    if (w == 0) {
+      uint32_t base = 0;
+      for (int i = 0; i < chunks; i += 64) {
+        uint32_t t = i + lane < chunks ? csum[i + lane] : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const uint32_t o = __shfl_up(t, d);
+          if (lane >= d) t += o;
+        }
+        t += base;
+        if (i + lane < chunks) csum[i + lane] = t;
+        base = __builtin_amdgcn_readlane(t, 63);
+      }
+    }
+    __syncthreads();
+    total = __builtin_amdgcn_readfirstlane(csum[chunks - 1]);
   }
-  s = __builtin_amdgcn_readfirstlane(s);
-  before = uniform(before);
-  Seq sq = sequence(c, s);
-  int T = tiles_of(sq), hb = (int)quotient(from - before, T);
-  int64_t item0 = before + (int64_t)hb * T;  // the item's first tile in the list
-  for (int64_t at = from; at < to;) {
-    const int kvh = hb % c.kv_heads, rb = hb / c.kv_heads;
-    const int64_t item1 = item0 + T;
-    const int b0 = (int)quotient(item0, run), b1 = (int)quotient(item1 - 1, run);
+  const uint32_t run = max((total + gridDim.x - 1) >> a.blocks_log2, (uint32_t)NW);
+  uint32_t at = min(run * blockIdx.x, total);
+  const uint32_t to = min(at + run, total);
+  if (at >= to) return;
+  // the sequence that holds the run's first tile, and the list's tiles before it
+  uint32_t before = 0;
+  if (chunks > 1) {
+    int ch = 0;
+    for (int i = 0; i < chunks; i += 64) ch += __popcll(__ballot(i + lane < chunks && csum[min(i + lane, chunks - 1)] <= at));
+    if (ch) before = __builtin_amdgcn_readfirstlane(csum[ch - 1]);
+    if (ch != held) hold(ch);
+  }
+  int j = __ffsll((unsigned long long)__ballot(before + upto > at)) - 1;
+  before += __builtin_amdgcn_readlane(upto, j) - __builtin_amdgcn_readlane(own, j);
+  Seq sq = held_seq(j);
+  int s = 64 * held + j, T = tiles_of(sq), hb = (int)((at - before) / T);
+  uint32_t item0 = before + hb * T;  // the item's first tile in the list
+  for (;;) {
+    int rb = 0, kvh = hb;
+    while (kvh >= kv_heads) {
+      kvh -= kv_heads;
+      ++rb;
+    }
     decode_item<D, BF, RT>(a, smem, ml, pcare, &last_block, s, sq, kvh, rb, first_key(sq), (int)(at - item0),
-                           (int)(min(item1, to) - item0), b0, b1, lane, w, n, g);
-    at = item1;
-    item0 = item1;
-    if (++hb == H) {
-      hb = 0;
-      do {
-        if (++s >= c.seqs) return;
-        sq = sequence(c, s);
-        T = tiles_of(sq);
-      } while (T == 0);
-    }
+                           (int)(min(item0 + T, to) - item0), item0, T, run, lane, w, n, g);
+    at = item0 = item0 + T;
+    if (at >= to) break;
+    if (++hb < H) continue;
+    hb = 0;
+    do {  // (a later sequence has tiles, since the list goes on)
+      if ((++s >> 6) != held) hold(s >> 6);
+      sq = held_seq(s & 63);
+      T = tiles_of(sq);
+    } while (T == 0);
   }
 }
 
@@ -490,7 +515,7 @@ hipError_t append_x(const AppendArgs& a, int type, int x_type, hipStream_t s) {
 
 template <int D, bool BF>
 hipError_t decode_d(const AttnArgs& a, const DecodePlan& p, hipStream_t s) {
-  const dim3 grid((uint32_t)p.blocks);
+  const dim3 grid(1u << p.blocks_log2);
   if (p.row_tiles == 1) k_attn_decode<D, BF, 1><<<grid, 64 * NW, 0, s>>>(a);
   else if (p.row_tiles == 2) k_attn_decode<D, BF, 2><<<grid, 64 * NW, 0, s>>>(a);
   else k_attn_decode<D, BF, 4><<<grid, 64 * NW, 0, s>>>(a);
@@ -504,12 +529,18 @@ DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_
   const int rows = group * max_new;
   p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
   p.row_blocks = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
-  // a block per CU, each with a tile per wave at least
+  // A block per CU, or two where a block would have more than one item to go through and registers for two are there (one row
+  // tile): the second works while the first goes from one item to the next, but an item in more parts takes longer to
+  // join. us with one / two: 512 items of 500-16000 keys 208 / 196, 2048 items (dim 64) 437 / 382, 1600 items of 100-3000 keys
+  // 216 / 182; 128 items 29 / 29 and 51 / 52, 8 items of 131071 keys 98 / 107, 1 item of a million 109 / 126. Fewer (a power of two)
+  // where they would not have a tile per wave.
   const int64_t items = (int64_t)seqs * kv_heads * p.row_blocks, tiles = items * (max_kv / 32 + 2);
-  p.min_run = NW;
-  p.blocks = (int)std::max<int64_t>(1, std::min<int64_t>(256, (tiles + NW - 1) / NW));
+  const int most = items > 256 && p.row_tiles == 1 ? 9 : 8;
+  p.blocks_log2 = 0;
+  while (p.blocks_log2 < most && ((int64_t)NW << p.blocks_log2) < tiles) ++p.blocks_log2;
   p.count_bytes = ((size_t)items * 4 + 255) & ~(size_t)255;
-  p.part_bytes = (size_t)p.blocks * 2 * p.row_tiles * 16 * (head_dim + 2) * 4;
+  p.part_bytes = ((size_t)1 << p.blocks_log2) * 2 * p.row_tiles * 16 * (head_dim + 2) * 4;
+  p.most_keys = (int)std::min<int64_t>(1 << 30, ((int64_t)1 << 36) / std::max<int64_t>(items, 1) / 2 - 64);
   return p;
 }
 

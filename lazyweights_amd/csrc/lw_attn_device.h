@@ -54,6 +54,12 @@ __device__ __forceinline__ uint2 read_tr(const uint16_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS4*)p));
 }
 
+// 16 bytes per lane from src to LDS, lane l's at dst + 16 l (dst the same in every lane)
+__device__ __forceinline__ void copy_lds16(const uint16_t* src, uint16_t* dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
+                                   (__attribute__((address_space(3))) uint32_t*)dst, 16, 0, 0);
+}
+
 // v combined with lane ^ 32's (and ^ 16's)
 __device__ __forceinline__ uint2 swap32(uint32_t v) {
   const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);

@@ -7,12 +7,6 @@ namespace {
 
 // ── prompt ──────────────────────────────────────────────────────────────────────────────────────────────────────────
 
-// 16 bytes per lane from src to LDS, lane l's at dst + 16 l (dst the same in every lane)
-__device__ __forceinline__ void copy_lds16(const uint16_t* src, uint16_t* dst) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src,
-                                   (__attribute__((address_space(3))) uint32_t*)dst, 16, 0, 0);
-}
-
 // every wave's copies have arrived, and every wave is done with what it read
 __device__ __forceinline__ void arrived() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -49,21 +43,23 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const AttnArgs a) {
   const int R = sq.rows * a.group, r0 = (tile - first_tile(s)) * ROWS;
   if (r0 < 0 || r0 >= R) return;
   const int past = sq.len - sq.rows;
-  const int pos_last = past + (min(r0 + ROWS, R) - 1) / a.group, pos_first = past + r0 / a.group;
+  const Divisor by_group = a.by_group;
+  const int pos_last = past + by_group(min(r0 + ROWS, R) - 1), pos_first = past + by_group(r0);
   const int hi = min(pos_last + 1, sq.len);
   const int lo = a.window > 0 ? max(0, pos_first - a.window + 1) & ~63 : 0;
   const int tiles = hi > lo ? (hi - lo + 63) / 64 : 0;
 
   // this wave's rows
-  const int row = r0 + 32 * w + n, tok = row / a.group, head = kvh * a.group + row % a.group;
+  const int row = r0 + 32 * w + n, tok = by_group(row), head = kvh * a.group + row - tok * a.group;
   const int pos = row < R ? past + tok : -1;
-  const int wlo = past + min(r0 + 32 * w, R - 1) / a.group, whi = past + min(r0 + 32 * w + 31, R - 1) / a.group;
+  const int wlo = past + by_group(min(r0 + 32 * w, R - 1)), whi = past + by_group(min(r0 + 32 * w + 31, R - 1));
   const bool full = r0 + 32 * w + 32 <= R, empty = r0 + 32 * w >= R;
+  const u32x4 flip = (u32x4)(uint32_t)__builtin_amdgcn_readfirstlane(a.q_flip);
   u32x4 qf[2 * C];
 #pragma unroll
   for (int i = 0; i < 2 * C; ++i)
     qf[i] = row < R ? *reinterpret_cast<const u32x4*>(a.q + (int64_t)(sq.row0 + tok) * a.ldq + (int64_t)head * D + 16 * i + 8 * g) ^
-                          a.q_flip
+                          flip
                     : (u32x4)0;
 
   const int lrow = ((lane & 15) - 4 * (lane >> 4)) & 15;  // the row of its block that this lane copies
