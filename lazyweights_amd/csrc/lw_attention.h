@@ -61,14 +61,15 @@ struct AttnArgs {
   // the decode kernel's workspace and division (DecodePlan)
   float* part;
   uint32_t* count;
-  int row_blocks, blocks_log2, most_keys;
+  int row_blocks, blocks_log2, most_keys, whole;
 };
 
 // How the decode kernel divides a batch: row_tiles tiles of 16 (token, head) rows per item, row_blocks items for a
 // sequence's key-value head, and a power of two of blocks. The list of all items' tiles of 32 keys is counted in 32 bits:
 // most_keys is the most of a sequence that keeps it there (2^31 tiles in all).
 struct DecodePlan {
-  int row_tiles, row_blocks, blocks_log2, most_keys;
+  int row_tiles, row_blocks, blocks, blocks_log2, most_keys;
+  bool whole;  // a block per item, of 8 waves
   size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
 };
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);

@@ -99,7 +99,7 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   a.window = (int)std::min<long long>(window, kMostRows);
   a.part = nullptr;
   a.count = nullptr;
-  a.row_blocks = a.blocks_log2 = a.most_keys = 0;
+  a.row_blocks = a.blocks_log2 = a.most_keys = a.whole = 0;
   return 0;
 }
 
@@ -173,6 +173,7 @@ int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(batch->workspace) + p.count_bytes);
   a.row_blocks = p.row_blocks;
   a.blocks_log2 = p.blocks_log2;
+  a.whole = p.whole;
   a.most_keys = p.most_keys;
   return launched(fn, lw::launch_attn_decode(a, p, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
 }

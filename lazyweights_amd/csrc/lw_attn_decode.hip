@@ -78,11 +78,9 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
 
 // ── decode ──────────────────────────────────────────────────────────────────────────────────────────────────────────
 
-constexpr int NW = 4;  // waves of a block
-
 // Tiles [t_from, t_to) of the item (s, kvh, rb), whose keys start at `lo` and whose T tiles are the list's from item0 on; a block
-// has `run` tiles of the list.
-template <int D, bool BF, int RT>
+// has `run` tiles of the list (or a whole item, which is joined by nobody else).
+template <int D, bool BF, int RT, int NW>
 __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, float* ml, float* pcare, int* last_block, int s, const Seq& sq,
                                             int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0, int T,
                                             uint32_t run, int lane, int w, int n, int g) {
@@ -401,7 +399,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 // keys as the sequence's rows see together; the launch's blocks take equal runs of the list's tiles, whatever the lengths.
 // Within a run, a block's waves take the tiles of an item in turn, each on its own (no barrier in the loop), and join at
 // the item's end. An item that lies in several runs is joined, in their order, by the block that ends last.
-template <int D, bool BF, int RT>
+template <int D, bool BF, int RT, int NW>
 __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void k_attn_decode(const AttnArgs a) {
   __shared__ __align__(16) uint8_t smem[NW * 32 * D * 2];  // V tiles of the waves; after the loop their sums
   __shared__ float ml[NW * 16 * RT * 2];
@@ -415,6 +413,13 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void k_attn_decode(const 
   // the zeros
   auto first_key = [&](const Seq& q) { return a.window > 0 ? max(0, q.len - q.rows - a.window + 1) & ~31 : 0; };
   auto tiles_of = [&](const Seq& q) { return q.rows ? max((q.len - first_key(q) + 31) >> 5, 1) : 0; };
+  if (a.whole) {
+    const int s = (int)blockIdx.x / H, hb = (int)blockIdx.x - s * H, rb = hb / kv_heads;
+    const Seq sq = sequence(c, s);
+    const int T = tiles_of(sq);
+    if (T) decode_item<D, BF, RT, NW>(a, smem, ml, pcare, &last_block, s, sq, hb - rb * kv_heads, rb, first_key(sq), 0, T, 0, T, T, lane, w, n, g);
+    return;
+  }
   // the sequences are held 64 at a time, one per lane, with their tiles and those up to theirs
   Seq mine;
   uint32_t own, upto;
@@ -486,7 +491,7 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void k_attn_decode(const 
       kvh -= kv_heads;
       ++rb;
     }
-    decode_item<D, BF, RT>(a, smem, ml, pcare, &last_block, s, sq, kvh, rb, first_key(sq), (int)(at - item0),
+    decode_item<D, BF, RT, NW>(a, smem, ml, pcare, &last_block, s, sq, kvh, rb, first_key(sq), (int)(at - item0),
                            (int)(min(item0 + T, to) - item0), item0, T, run, lane, w, n, g);
     at = item0 = item0 + T;
     if (at >= to) break;
@@ -515,10 +520,11 @@ hipError_t append_x(const AppendArgs& a, int type, int x_type, hipStream_t s) {
 
 template <int D, bool BF>
 hipError_t decode_d(const AttnArgs& a, const DecodePlan& p, hipStream_t s) {
-  const dim3 grid(1u << p.blocks_log2);
-  if (p.row_tiles == 1) k_attn_decode<D, BF, 1><<<grid, 64 * NW, 0, s>>>(a);
-  else if (p.row_tiles == 2) k_attn_decode<D, BF, 2><<<grid, 64 * NW, 0, s>>>(a);
-  else k_attn_decode<D, BF, 4><<<grid, 64 * NW, 0, s>>>(a);
+  const dim3 grid((uint32_t)p.blocks);
+  if (p.row_tiles == 1 && p.whole) k_attn_decode<D, BF, 1, 8><<<grid, 512, 0, s>>>(a);
+  else if (p.row_tiles == 1) k_attn_decode<D, BF, 1, 4><<<grid, 256, 0, s>>>(a);
+  else if (p.row_tiles == 2) k_attn_decode<D, BF, 2, 4><<<grid, 256, 0, s>>>(a);
+  else k_attn_decode<D, BF, 4, 4><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -536,8 +542,13 @@ DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_
   // where they would not have a tile per wave.
   const int64_t items = (int64_t)seqs * kv_heads * p.row_blocks, tiles = items * (max_kv / 32 + 2);
   const int most = items > 256 && p.row_tiles == 1 ? 9 : 8;
+  // A block of 8 waves per item: where every wave has one tile at most, nothing is left to join between blocks (us against
+  // runs: 201 keys 8.4 / 13.7, but 778 keys, four tiles after another, 15.6 / 12.9); and where there are many items, none long
+  // (1600 items of 100-3000 keys 175 / 182, 1024 of 628-3033 130 / 141; 512 of 500-16000 270 / 198).
+  p.whole = p.row_tiles == 1 && items <= 1 << 20 && (max_kv <= 256 || (items >= 1024 && max_kv <= 4096));
   p.blocks_log2 = 0;
-  while (p.blocks_log2 < most && ((int64_t)NW << p.blocks_log2) < tiles) ++p.blocks_log2;
+  while (p.blocks_log2 < most && ((int64_t)4 << p.blocks_log2) < tiles) ++p.blocks_log2;
+  p.blocks = p.whole ? (int)items : 1 << p.blocks_log2;
   p.count_bytes = ((size_t)items * 4 + 255) & ~(size_t)255;
   p.part_bytes = ((size_t)1 << p.blocks_log2) * 2 * p.row_tiles * 16 * (head_dim + 2) * 4;
   p.most_keys = (int)std::min<int64_t>(1 << 30, ((int64_t)1 << 36) / std::max<int64_t>(items, 1) / 2 - 64);

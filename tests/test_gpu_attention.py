@@ -526,3 +526,32 @@ def test_prompt_of_many_rows(gpu, lib, case):
     seen[250:min(300, 250 + window) if window else 300] = True
     assert torch.isnan(y[seen]).all()
     check(torch, y[~seen], [t[~seen] for t in ref], dtype, True)
+
+
+BATCHES = [
+    # layout, sequences, longest, bound on the length, new tokens: forms of the launch by items (sequences x kv heads), bound
+    ((2, 1, 64), 301, 40, 5000, 2),    # 301 items, runs over more sequences than lanes
+    ((8, 8, 96), 70, 700, 700, 1),     # 560 items, more blocks than CUs
+    ((16, 8, 128), 130, 600, 600, 1),  # 1040 items, one block each
+    ((4, 2, 128), 3, 250, 250, 4),     # short: one block each
+    ((64, 2, 96), 5, 2000, 2000, 1),   # two row tiles
+    ((8, 4, 64), 1000, 3, 9000, 1),    # most sequences empty or of a token, runs of a few tiles
+]
+
+
+@pytest.mark.parametrize("case", BATCHES, ids=str)
+def test_decode_batches(gpu, lib, case):
+    import random
+
+    import torch
+    layout, seqs, longest, bound, most = case
+    rng = random.Random(seqs)
+    lengths = [(rng.randrange(0 if seqs > 60 else 1, most + 1), rng.choice((0, 1, 31, 32, 33, longest - 5, rng.randrange(longest))))
+               for _ in range(seqs)]
+    lengths = [(n, max(0, min(o, longest - n))) for n, o in lengths]
+    k, v, table, q_start, kv_len, q = make(torch, layout, 16, torch.float16, lengths, 28, width=-(-bound // 16))
+    cache, batch = build(torch, layout, k, v, table, q_start, kv_len, most, bound)
+    ref = reference(torch, k, v, table, lengths, q, 0, layout[2] ** -0.5)
+    y = torch.full(q.shape, float("nan"), device="cuda")
+    for _ in range(2):
+        check(torch, cache.attend_decode(batch, q, out=y.fill_(float("nan"))), ref, torch.float16, False)
