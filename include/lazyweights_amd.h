@@ -229,8 +229,8 @@ typedef struct lw_kv_cache {
  * between replays of a captured call) without the host reading them. What the arrays hold is kept in range by the
  * kernels: rows lie in [0, tokens), lengths in the page table, and a page number outside [0, pages) stands for a page
  * that is not there: nothing is appended to it and no row sees its positions. workspace: lw_attn_workspace() bytes,
- * aligned to 16, zero before its first use; calls leave it ready for the next one. Calls that share one must not
- * overlap. */
+ * aligned to 16, zero before its first use; calls leave it ready for the next one with the same seqs, max_new, max_kv, heads and
+ * cache shape (zero it before others use it). Calls that share one must not overlap. lw_attn_prompt also works without. */
 typedef struct lw_batch {
   int32_t seqs, tokens, max_new, max_kv;
   const int32_t* q_start;    /* [seqs + 1] */

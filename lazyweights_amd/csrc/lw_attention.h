@@ -62,6 +62,7 @@ struct AttnArgs {
   float* part;
   uint32_t* count;
   int row_blocks, blocks_log2, most_keys, whole;
+  int splits;  // the prompt kernel's: blocks that share the keys of a row tile, their sums in `part`
 };
 
 // How the decode kernel divides a batch: row_tiles tiles of 16 (token, head) rows per item, row_blocks items for a
@@ -73,6 +74,13 @@ struct DecodePlan {
   size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
 };
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);
+
+// The prompt kernel's row tiles of 128 (token, head) rows of a key-value head, and into how many blocks the keys of each are shared
+// out, with a workspace of `slots` slots of prompt_slot_bytes() each (kPromptSlots are of use).
+constexpr int kPromptSlots = 512;
+int64_t prompt_items(int seqs, int kv_heads, int group, int tokens);
+size_t prompt_slot_bytes(int head_dim);
+int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots);
 
 hipError_t launch_append(const AppendArgs& a, int head_dim, int type, int x_type, hipStream_t s);
 hipError_t launch_attn_decode(const AttnArgs& a, const DecodePlan& p, int head_dim, int type, hipStream_t s);

@@ -100,6 +100,7 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   a.part = nullptr;
   a.count = nullptr;
   a.row_blocks = a.blocks_log2 = a.most_keys = a.whole = 0;
+  a.splits = 1;
   return 0;
 }
 
@@ -110,7 +111,9 @@ extern "C" {
 long long lw_attn_workspace(const lw_kv_cache* cache, const lw_batch* batch, int heads) {
   const std::string bad = check(cache, batch, heads);
   if (!bad.empty()) return refuse("lw_attn_workspace", bad);
-  if (batch->seqs == 0 || batch->max_new > 16) return 0;
+  if (batch->seqs == 0) return 0;
+  if (batch->max_new > 16)  // (a row tile's keys are shared out where there are three times 1024 and more)
+    return batch->max_kv < 3 * 1024 ? 0 : (long long)(lw::kPromptSlots * lw::prompt_slot_bytes(cache->head_dim));
   const lw::DecodePlan p = lw::decode_plan(batch->seqs, cache->kv_heads, heads / cache->kv_heads, cache->head_dim,
                                            batch->max_new, batch->max_kv);
   return (long long)(p.count_bytes + p.part_bytes);
@@ -186,6 +189,18 @@ int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
   if (rc) return rc < 0 ? -1 : 0;
   if (((long long)batch->tokens * a.group / 128 + batch->seqs) * cache->kv_heads > kMostBlocks)
     return refuse(fn, "more tokens than a launch can take");
+  if (batch->workspace && (reinterpret_cast<uintptr_t>(batch->workspace) & 15)) return refuse(fn, "workspace not aligned to 16");
+  if (batch->workspace) {  // (past the counters of lw_attn_decode, if the batch may go there)
+    size_t skip = 0;
+    if (batch->max_new <= 16)
+      skip = lw::decode_plan(batch->seqs, cache->kv_heads, a.group, cache->head_dim, std::max(batch->max_new, 1), batch->max_kv)
+                 .count_bytes;
+    a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(batch->workspace) + skip);
+    const long long bytes = batch->workspace_bytes - (long long)skip;
+    if (bytes > 0)
+      a.splits = lw::prompt_splits(batch->seqs, cache->kv_heads, a.group, batch->tokens, batch->max_kv,
+                                   bytes / (long long)lw::prompt_slot_bytes(cache->head_dim));
+  }
   return launched(fn, lw::launch_attn_prompt(a, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
 }
 

@@ -1,4 +1,6 @@
 // Attention of whole prompts, or chunks of them, over a paged key-value cache.
+#include <algorithm>
+
 #include "lw_attn_device.h"
 
 namespace lw {
@@ -13,6 +15,36 @@ __device__ __forceinline__ void arrived() {
   __syncthreads();
 }
 
+// The ROWS rows (token, head) of a sequence that a block has, and the keys [lo, hi) that they see together, in `tiles` tiles of 64.
+struct RowTile {
+  Seq sq;
+  int s, r0, rows, lo, hi, tiles;
+  // the tiles that each of `splits` blocks takes (eight at least): the first one has some wherever there are any
+  __device__ __forceinline__ int tiles_each(int splits) const { return splits > 1 ? max((tiles + splits - 1) / splits, 8) : tiles; }
+};
+template <int ROWS>
+__device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int tile) {
+  const KvView& c = a.c;
+  const int tokens = c.tokens, group = a.group;
+  // sequence s owns tiles from q_start[s] group / ROWS + s on: at least as many as its rows take
+  auto first_tile = [&](int i) { return (int)((int64_t)clampi(c.q_start[i], 0, tokens) * group / ROWS) + i; };
+  RowTile t;
+  t.s = __builtin_amdgcn_readfirstlane(last_at_most(c.seqs, tile, first_tile));
+  t.sq = sequence(c, t.s);
+  const int R = t.sq.rows * group, past = t.sq.len - t.sq.rows;
+  t.r0 = (tile - first_tile(t.s)) * ROWS;
+  t.rows = t.r0 < 0 ? 0 : min(R - t.r0, ROWS);
+  t.lo = t.hi = t.tiles = 0;
+  if (t.rows > 0) {
+    const Divisor by_group = a.by_group;
+    const int first = past + by_group(t.r0), last = past + by_group(t.r0 + t.rows - 1);
+    t.hi = min(last + 1, t.sq.len);
+    t.lo = a.window > 0 ? max(0, first - a.window + 1) & ~63 : 0;
+    t.tiles = t.hi > t.lo ? (t.hi - t.lo + 63) / 64 : 0;
+  }
+  return t;
+}
+
 // A block: W waves, each 32 rows (token, head) of one key-value head of a sequence, over the keys they see in tiles of 64.
 // K and V tiles lie in LDS as [16-key block][D / 8 chunks][16 slots][8 dims], key k of a block in slot (k + 4 chunk) & 15:
 // the score product's operand reads (32 keys of a chunk) and the transposed reads of V (4 keys of 4 chunks) are both free
@@ -22,6 +54,9 @@ __device__ __forceinline__ void arrived() {
 // Of 8 waves, two share a SIMD, and all meet once per tile: so that one's softmax runs beside the other's products, the
 // last four work through a tile in another order, the second product of the tile before first (V has four buffers).
 // 4 waves leave room for a second block on the CU, which runs at its own pace.
+//
+// Where there are few rows (AttnArgs::splits > 1), the key tiles of a block's rows are shared out to up to `splits` blocks, which
+// leave their maxima and sums in slots of the workspace, lane by lane, for k_attn_join.
 template <int D, bool BF, int NP, int W>
 __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const AttnArgs a) {
   constexpr int C = D / 32, ROWS = 32 * W, BLK = D * 16;  // BLK: elements of a 16-key block
@@ -33,21 +68,18 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const AttnArgs a) {
   __shared__ int any_bad;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
   const KvView& c = a.c;
-  const int kvh = blockIdx.x % c.kv_heads, tile = (int)(gridDim.x / c.kv_heads) - 1 - (int)(blockIdx.x / c.kv_heads);
-  // sequence s owns tiles from q_start[s] group / ROWS + s on: at least as many as its rows take
-  auto first_tile = [&](int i) {
-    return (int)((int64_t)clampi(c.q_start[i], 0, c.tokens) * a.group / ROWS) + i;
-  };
-  const int s = __builtin_amdgcn_readfirstlane(last_at_most(c.seqs, tile, first_tile));
-  const Seq sq = sequence(c, s);
-  const int R = sq.rows * a.group, r0 = (tile - first_tile(s)) * ROWS;
-  if (r0 < 0 || r0 >= R) return;
+  const int splits = W == 4 ? a.splits : 1, unit = blockIdx.x / c.kv_heads, kvh = blockIdx.x - unit * c.kv_heads;
+  const int tile = (int)(gridDim.x / c.kv_heads) / splits - 1 - unit / splits, share = unit % splits;
+  const RowTile rt = row_tile<ROWS>(a, tile);
+  if (rt.rows <= 0) return;
+  const Seq& sq = rt.sq;
+  const int s = rt.s, R = sq.rows * a.group, r0 = rt.r0;
   const int past = sq.len - sq.rows;
   const Divisor by_group = a.by_group;
-  const int pos_last = past + by_group(min(r0 + ROWS, R) - 1), pos_first = past + by_group(r0);
-  const int hi = min(pos_last + 1, sq.len);
-  const int lo = a.window > 0 ? max(0, pos_first - a.window + 1) & ~63 : 0;
+  const int each = W == 4 ? rt.tiles_each(splits) : rt.tiles;
+  const int lo = rt.lo + 64 * each * share, hi = min(rt.hi, lo + 64 * each);
   const int tiles = hi > lo ? (hi - lo + 63) / 64 : 0;
+  if (share > 0 && tiles == 0) return;
 
   // this wave's rows
   const int row = r0 + 32 * w + n, tok = by_group(row), head = kvh * a.group + row - tok * a.group;
@@ -254,6 +286,18 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < C; ++d) o[d] = (f16x16)0.f;
   }
+  if (W == 4 && rt.tiles > each) {  // its share: m, l, then four sums at a time, lane by lane
+    float* z = a.part + ((int64_t)(tile * c.kv_heads + kvh) * splits + share) * (ROWS * (D + 4)) + w * 32 * (D + 4) + lane;
+    z[0] = m;
+    z[64] = l;
+    f4v* zo = reinterpret_cast<f4v*>(z - lane + 128) + lane;
+#pragma unroll
+    for (int d = 0; d < C; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        zo[64 * (4 * d + j)] = (f4v){o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]};
+    return;
+  }
   if (row >= R) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int64_t at = (int64_t)(sq.row0 + tok) * a.ldo + (int64_t)head * D + 4 * g;
@@ -268,9 +312,40 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const AttnArgs a) {
     }
 }
 
+// Joins the shares of row tiles that k_attn_prompt left in the workspace: block (item, d) the dims 32 d .. 32 d + 31 of a row tile
+// of a key-value head, its waves and lanes as there.
+template <int D>
+__global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a) {
+  constexpr int C = D / 32;
+  const KvView& c = a.c;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, g = lane >> 5;
+  const int item = blockIdx.x / C, d = blockIdx.x - item * C, tile = item / c.kv_heads, kvh = item - tile * c.kv_heads;
+  const RowTile rt = row_tile<128>(a, tile);
+  const int each = rt.tiles_each(a.splits), row = 32 * w + n;
+  if (rt.tiles <= each || row >= rt.rows) return;
+  const int shares = (rt.tiles + each - 1) / each;
+  const float* z = a.part + (int64_t)item * a.splits * (128 * (D + 4)) + w * 32 * (D + 4) + lane;
+  float m = -INFINITY, l = 0.f;
+  f4v o[4] = {(f4v)0.f, (f4v)0.f, (f4v)0.f, (f4v)0.f};
+#pragma unroll 4
+  for (int i = 0; i < shares; ++i) {
+    const float* p = z + (int64_t)i * (128 * (D + 4));
+    const f4v* po = reinterpret_cast<const f4v*>(p - lane + 128) + lane + 64 * 4 * d;
+    const float m2 = p[0], up = fmaxf(m, m2), base = up == -INFINITY ? 0.f : up, x = pow2(m - base), y = pow2(m2 - base);
+    m = up;
+    l = l * x + p[64] * y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * x + po[64 * j] * y;
+  }
+  const int tok = a.by_group(rt.r0 + row), head = kvh * a.group + rt.r0 + row - tok * a.group;
+  const int64_t at = (int64_t)(rt.sq.row0 + tok) * a.ldo + (int64_t)head * D + 32 * d + 4 * g;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) store4(a.out_type, a.out, at + 8 * j, normal(o[j], l));
+}
+
 template <int D, bool BF, int W>
-hipError_t prompt_w(const AttnArgs& a, hipStream_t s) {
-  const dim3 grid((uint32_t)(((int64_t)a.c.tokens * a.group / (32 * W) + a.c.seqs) * a.c.kv_heads));
+hipError_t prompt_w(const AttnArgs& a, int splits, hipStream_t s) {
+  const dim3 grid((uint32_t)(((int64_t)a.c.tokens * a.group / (32 * W) + a.c.seqs) * a.c.kv_heads * splits));
   if (a.out_type == 0) k_attn_prompt<D, BF, BF ? 3 : 2, W><<<grid, 64 * W, 0, s>>>(a);
   else k_attn_prompt<D, BF, 1, W><<<grid, 64 * W, 0, s>>>(a);
   return hipGetLastError();
@@ -281,10 +356,31 @@ hipError_t prompt_d(const AttnArgs& a, hipStream_t s) {
   // blocks for every CU (15999 tokens of 32 heads 2137 us against 2241), slower below (766 blocks of ragged prompts 148
   // against 133, 125 blocks 133 against 107)
   const int64_t blocks = (int64_t)a.c.tokens * a.group / 256 * a.c.kv_heads;
-  return blocks >= 1024 ? prompt_w<D, BF, 8>(a, s) : prompt_w<D, BF, 4>(a, s);
+  if (blocks >= 1024) return prompt_w<D, BF, 8>(a, 1, s);
+  hipError_t e = prompt_w<D, BF, 4>(a, a.splits, s);
+  if (e == hipSuccess && a.splits > 1) {
+    k_attn_join<D><<<dim3((uint32_t)prompt_items(a.c.seqs, a.c.kv_heads, a.group, a.c.tokens) * (D / 32)), 256, 0, s>>>(a);
+    e = hipGetLastError();
+  }
+  return e;
 }
 
 }  // namespace
+
+int64_t prompt_items(int seqs, int kv_heads, int group, int tokens) {
+  return ((int64_t)tokens * group / 128 + seqs) * kv_heads;
+}
+
+size_t prompt_slot_bytes(int head_dim) { return (size_t)128 * (head_dim + 4) * 4; }
+
+int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots) {
+  // Two blocks per CU, of 1024 keys and more, where that makes three at least of every row tile's: us with / without, the join
+  // included, 64 tokens after 20000 59 / 504, 500 after 3000 52 / 89; two shares of 256 row tiles gain nothing (1000 tokens
+  // after 9001 100 / 106, their sums' way through memory takes 13), nor do few keys (700 tokens 27 / 25).
+  const int64_t items = prompt_items(seqs, kv_heads, group, tokens);
+  const int64_t splits = std::min<int64_t>(std::min<int64_t>(kPromptSlots, slots) / items, max_kv / 1024);
+  return splits < 3 ? 1 : (int)splits;
+}
 
 hipError_t launch_attn_prompt(const AttnArgs& a, int head_dim, int type, hipStream_t s) {
   if (head_dim == 64) return type == 2 ? prompt_d<64, true>(a, s) : prompt_d<64, false>(a, s);

@@ -555,3 +555,53 @@ def test_decode_batches(gpu, lib, case):
     y = torch.full(q.shape, float("nan"), device="cuda")
     for _ in range(2):
         check(torch, cache.attend_decode(batch, q, out=y.fill_(float("nan"))), ref, torch.float16, False)
+
+
+SHARED_KEYS = [
+    # layout, page, type, out, (new, old) per sequence, window: few rows, so that blocks share a row tile's keys
+    ((4, 2, 128), 16, "float16", "float32", [(20, 3000), (1, 5000), (130, 700), (0, 9), (33, 0)], 0),
+    ((8, 1, 96), 64, "bfloat16", "bfloat16", [(40, 6001), (17, 300)], 0),
+    ((4, 4, 64), 8, "float16", "float16", [(300, 4000), (5, 100)], 3500),
+    ((2, 2, 128), 32, "bfloat16", "float32", [(129, 4000)], 300),
+    ((3, 1, 64), 16, "float16", "float32", [(18, 511), (2, 20000)], 0),
+]
+
+
+@pytest.mark.parametrize("case", SHARED_KEYS, ids=str)
+def test_prompt_of_few_rows_and_many_keys(gpu, lib, case):
+    import torch
+    layout, page, dtype, out, lengths, window = case
+    dtype, out = getattr(torch, dtype), getattr(torch, out)
+    unmapped = [(0, 300 // page)]
+    k, v, table, q_start, kv_len, q = make(torch, layout, page, dtype, lengths, 29, unmapped=unmapped)
+    most = max(n + o for n, o in lengths)
+    cache, batch = build(torch, layout, k, v, table, q_start, kv_len, max(n for n, _ in lengths), most)
+    assert batch.workspace.numel() > 0
+    ref = reference(torch, k, v, table, lengths, q, window, layout[2] ** -0.5)
+    y = torch.full(q.shape, float("nan"), dtype=out, device="cuda")
+    for _ in range(3):
+        check(torch, cache.attend_prompt(batch, q, out=y.fill_(float("nan")), window=window), ref, dtype, True)
+    # the same without a workspace, in one block per row tile
+    batch.c.workspace, batch.c.workspace_bytes = None, 0
+    check(torch, cache.attend_prompt(batch, q, out=y.fill_(float("nan")), window=window), ref, dtype, True)
+
+
+def test_prompt_and_decode_share_a_workspace(gpu, lib):
+    """Few new tokens go through either call, one after the other, with the batch's workspace."""
+    import torch
+    layout, lengths = (8, 2, 128), [(3, 4000), (1, 900)]
+    k, v, table, q_start, kv_len, q = make(torch, layout, 16, torch.float16, lengths, 30)
+    cache, batch = build(torch, layout, k, v, table, q_start, kv_len, 3, 4003)
+    ref = reference(torch, k, v, table, lengths, q, 0, 128 ** -0.5)
+    for _ in range(3):
+        for call, prompt in ((cache.attend_decode, False), (cache.attend_prompt, True)):
+            check(torch, call(batch, q, out=torch.full(q.shape, float("nan"), device="cuda")), ref, torch.float16, prompt)
+    v[int(table[0, 250]), 1, 4, 9] = float("nan")  # the last position but two of the first sequence: hidden from one row
+    bad = [i for i in range(3) if 4000 + i >= 250 * 16 + 4]
+    assert not bad
+    v[int(table[0, 4001 // 16]), 1, 4001 % 16, 9] = float("nan")
+    for call, prompt in ((cache.attend_decode, False), (cache.attend_prompt, True)):
+        y = call(batch, q, out=torch.empty_like(q, dtype=torch.float32))
+        clean = [0, 3]
+        check(torch, y[clean], [t[clean] for t in ref], torch.float16, prompt)
+        assert torch.isnan(y[1:3, 4:, 9]).all() and not torch.isnan(y[1:3, :4]).any()
