@@ -157,18 +157,20 @@ __device__ __forceinline__ f2v get2(const float* p) {
 // bf16: 24; one: rounded)
 template <bool BF, int NP>
 __device__ __forceinline__ void split8(const float* p, u32x4* part) {
-  float r[8];
+  float r[8], minus = -1.f;
+  if (!BF) asm("" : "+s"(minus));  // (not seen as -1, so that a conversion and a difference are one instruction)
 #pragma unroll
   for (int i = 0; i < 8; ++i) r[i] = p[i];
 #pragma unroll
   for (int n = 0; n < NP; ++n) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t w = narrow2<BF>(r[2 * i], r[2 * i + 1]);
+      uint32_t w = narrow2<BF>(r[2 * i], r[2 * i + 1]);
       part[n][i] = w;
       if (n + 1 < NP) {
-        r[2 * i] -= wide<BF>((uint16_t)w);
-        r[2 * i + 1] -= wide<BF>((uint16_t)(w >> 16));
+        if (!BF) asm("" : "+v"(w));  // (what was rounded is read from the part: the compiler would round each value once more)
+        r[2 * i] = __builtin_fmaf(wide<BF>((uint16_t)w), minus, r[2 * i]);
+        r[2 * i + 1] = __builtin_fmaf(wide<BF>((uint16_t)(w >> 16)), minus, r[2 * i + 1]);
       }
     }
   }
