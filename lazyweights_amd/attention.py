@@ -52,7 +52,7 @@ class Batch:
     """`seqs` sequences whose new tokens are the rows of a call: q_start int32 [seqs + 1], kv_len int32 [seqs] (the lengths
     with the new tokens), page_table int32 [seqs, pages], all on the cache's GPU. max_new and max_kv bound every
     sequence's new tokens and length. A call's tensors may have more rows than q_start names; those are left alone. Holds
-    the workspace of attend_decode, so calls with one batch must not overlap."""
+    the workspace of attend_decode and attend_prompt, so calls with one batch must not overlap."""
 
     def __init__(self, cache, heads, q_start, kv_len, page_table, max_new, max_kv):
         seqs = kv_len.shape[0]

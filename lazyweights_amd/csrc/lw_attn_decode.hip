@@ -12,7 +12,10 @@ namespace {
 // q_out = R_i q, cache k = R_i k, cache v = v for the batch's new tokens, position i; R_i rotates pairs of the first `rot`
 // elements by the angles of row i of cos / sin: (x, y) -> (x c - y s, y c + x s), in 32 bits, rounded once when stored.
 // Pairs are elements j and j + rot / 2 ("halves") or 2 j and 2 j + 1 ("neighbours"). A thread takes 8 elements of a head:
-// 4 pairs, or 8 that are only copied.
+// 4 pairs, or 8 that are only copied, so that every load and store is 8 or 16 bytes and neighbouring threads' are adjacent.
+// Bound by memory: 16383 tokens of 32 + 8 + 8 heads of 128, fp32 in, 612 MB in 109 us (5.6 TB/s, two thirds of it read; a copy of
+// 1 GiB reaches 5.0). A few tokens are one pass of loads that depend on each other (the sequence, its length, the page):
+// 2.5 us for one token, 3.4 for 48 sequences, less than the 8 us that the host takes to make the call.
 template <int X, bool BF>  // X: type of q, k, v (LW_F32, LW_F16, LW_BF16)
 __device__ __forceinline__ f4v load4(const void* p, int64_t i) {
   if (X == 0) return *reinterpret_cast<const f4v*>(static_cast<const float*>(p) + i);
@@ -94,15 +97,24 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 
   const u32x4 flip = (u32x4)(uint32_t)__builtin_amdgcn_readfirstlane(a.q_flip);
   int pos[RT];
-  u32x4 qf[RT][C];
+  // q's operands: of one row tile in registers; of two in LDS (each wave's own, read per tile), since no registers for a second
+  // block per CU would be left (64 sequences of 100-3000 keys, 20 rows each: 115 us against 140)
+  constexpr bool QL = RT > 1;
+  u32x4 qr[QL ? 1 : C];
+  u32x4* ql = reinterpret_cast<u32x4*>(smem + (NW * 32 + w * RT * 16) * D * 2) + lane;
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + 16 * t + n, tok = by_group(r);
     pos[t] = r < R ? past + tok : 1 << 30;  // (past the last row: whatever, nothing is written)
     const uint16_t* q = a.q + (int64_t)(sq.row0 + tok) * a.ldq + (int64_t)(kvh * a.group + r - tok * a.group) * D + 8 * g;
 #pragma unroll
-    for (int i = 0; i < C; ++i) qf[t][i] = r < R ? *reinterpret_cast<const u32x4*>(q + 32 * i) ^ flip : (u32x4)0;
+    for (int i = 0; i < C; ++i) {
+      const u32x4 x = r < R ? *reinterpret_cast<const u32x4*>(q + 32 * i) ^ flip : (u32x4)0;
+      if (QL) ql[64 * (t * C + i)] = x;
+      else qr[QL ? 0 : i] = x;
+    }
   }
+  auto qf = [&](int t, int i) { return QL ? ql[64 * (t * C + i)] : qr[QL ? 0 : i]; };
   const int32_t* table = c.table + s * c.tstride;
   const uint16_t* kb = c.k + kvh * c.hstride + 8 * g;
   const uint16_t* vb = c.v + kvh * c.hstride + 8 * g;
@@ -154,7 +166,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
         for (int h = 0; h < 2; ++h) {
           f4v acc = (f4v)0.f;
 #pragma unroll
-          for (int i = 0; i < C; ++i) acc = mfma16<BF>(kf[h][i], qf[r][i], acc);
+          for (int i = 0; i < C; ++i) acc = mfma16<BF>(kf[h][i], qf(r, i), acc);
           sc[r][h] = acc;
         }
       uint32_t seen[2];
@@ -399,9 +411,19 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 // keys as the sequence's rows see together; the launch's blocks take equal runs of the list's tiles, whatever the lengths.
 // Within a run, a block's waves take the tiles of an item in turn, each on its own (no barrier in the loop), and join at
 // the item's end. An item that lies in several runs is joined, in their order, by the block that ends last.
+//
+// Each key and value is read once, for all rows of its key-value head: 2 x 2 x D bytes a key against 4 x D x rows operations, so
+// a few tens of rows are bound by memory and the matrix cores are used for their layout (an item of 4 rows fills a quarter of a
+// tile's columns, the matrix cores busy 5 % of the time). A wave has a tile's 32 keys and values in flight to registers (16 KB at D = 128)
+// while it works on the one before; V goes through LDS, its own, for the transposed reads. Times (us, and of what bytes):
+// 64 sequences of 500-16000 keys, 8 heads of 128: 196 (1.05 GB: 5.4 TB/s, of the 6.7 that a stream of reads reaches); one of
+// 131071: 97 (537 MB: 5.5); 4 x 5 tokens of 32 heads of 96 over 301-5003: 29 (101 MB); one of 778: 13. What separates the
+// first two from that stream are mostly the launch's ends, and the others are little else: the XCDs start up to 4 us after one
+// another, then come the lengths, a page number, its keys, and at the end the join of runs, each waiting for the one before.
 template <int D, bool BF, int RT, int NW>
-__global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void k_attn_decode(const AttnArgs a) {
-  __shared__ __align__(16) uint8_t smem[NW * 32 * D * 2];  // V tiles of the waves; after the loop their sums
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_decode(const AttnArgs a) {
+  // V tiles of the waves (after the loop their sums), then, of more than one row tile, q
+  __shared__ __align__(16) uint8_t smem[NW * (RT > 1 ? 32 + RT * 16 : 32) * D * 2];
   __shared__ float ml[NW * 16 * RT * 2];
   __shared__ float pcare[NW * 32 * 16];
   __shared__ uint32_t csum[1024];  // tiles of the sequences up to each 64th
@@ -523,8 +545,7 @@ hipError_t decode_d(const AttnArgs& a, const DecodePlan& p, hipStream_t s) {
   const dim3 grid((uint32_t)p.blocks);
   if (p.row_tiles == 1 && p.whole) k_attn_decode<D, BF, 1, 8><<<grid, 512, 0, s>>>(a);
   else if (p.row_tiles == 1) k_attn_decode<D, BF, 1, 4><<<grid, 256, 0, s>>>(a);
-  else if (p.row_tiles == 2) k_attn_decode<D, BF, 2, 4><<<grid, 256, 0, s>>>(a);
-  else k_attn_decode<D, BF, 4, 4><<<grid, 256, 0, s>>>(a);
+  else k_attn_decode<D, BF, 2, 4><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -533,15 +554,20 @@ hipError_t decode_d(const AttnArgs& a, const DecodePlan& p, hipStream_t s) {
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv) {
   DecodePlan p;
   const int rows = group * max_new;
-  p.row_tiles = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  // More than 16 rows: two row tiles per item, which share what is read, where there is much to read; else one, and more items,
+  // each sooner done (us with two / one: 8 sequences of 1000-8000 keys, 8 heads of 128, 20 rows 40 / 55, one of 20000, 64 rows
+  // 52 / 65; one of 500, 64 rows 22 / 15, 4 of 300-5000, 4 heads, 64 rows 33 / 29; at 160000 keys of all heads from 52 / 65 to
+  // 34 / 32). Four row tiles took 54 and 97 in the cases of 500 and 20000 keys: no registers for a second block, and a join of
+  // all their sums by one.
+  p.row_tiles = rows <= 16 || (int64_t)seqs * kv_heads * max_kv < 1 << 17 ? 1 : 2;
   p.row_blocks = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
-  // A block per CU, or two where a block would have more than one item to go through and registers for two are there (one row
-  // tile): the second works while the first goes from one item to the next, but an item in more parts takes longer to
-  // join. us with one / two: 512 items of 500-16000 keys 208 / 196, 2048 items (dim 64) 437 / 382, 1600 items of 100-3000 keys
-  // 216 / 182; 128 items 29 / 29 and 51 / 52, 8 items of 131071 keys 98 / 107, 1 item of a million 109 / 126. Fewer (a power of two)
-  // where they would not have a tile per wave.
+  // A block per CU, or two where a block would have more than one item to go through: the second works while the first goes from
+  // one item to the next, but an item in more parts takes longer to join. us with one / two: 512 items of 500-16000 keys
+  // 208 / 196, 2048 items (dim 64) 437 / 382, 1600 items of 100-3000 keys 216 / 182, 512 of 100-3000 and two row tiles 130 / 115;
+  // 128 items 29 / 29 and 51 / 52, 8 items of 131071 keys 98 / 107, 1 item of a million 109 / 126. Fewer (a power of two) where
+  // they would not have a tile per wave.
   const int64_t items = (int64_t)seqs * kv_heads * p.row_blocks, tiles = items * (max_kv / 32 + 2);
-  const int most = items > 256 && p.row_tiles == 1 ? 9 : 8;
+  const int most = items > 256 ? 9 : 8;
   // A block of 8 waves per item: where every wave has one tile at most, nothing is left to join between blocks (us against
   // runs: 201 keys 8.4 / 13.7, but 778 keys, four tiles after another, 15.6 / 12.9); and where there are many items, none long
   // (1600 items of 100-3000 keys 175 / 182, 1024 of 628-3033 130 / 141; 512 of 500-16000 270 / 198).

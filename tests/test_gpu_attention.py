@@ -605,3 +605,48 @@ def test_prompt_and_decode_share_a_workspace(gpu, lib):
         clean = [0, 3]
         check(torch, y[clean], [t[clean] for t in ref], torch.float16, prompt)
         assert torch.isnan(y[1:3, 4:, 9]).all() and not torch.isnan(y[1:3, :4]).any()
+
+
+MANY_ROWS = [
+    # layout, page, type, out, new tokens per sequence, window; more than 16 rows (token, head) per key-value head and bounds
+    # of 2^17 positions of all heads, from which on an item has two row tiles
+    ((8, 2, 128), 16, "float16", "float32", [5, 16, 8, 0, 1], 0),
+    ((8, 1, 128), 64, "bfloat16", "float32", [3, 0, 4], 0),
+    ((64, 2, 96), 16, "float16", "float16", [1], 0),
+    ((12, 4, 96), 128, "bfloat16", "bfloat16", [16, 7, 11], 0),
+    ((40, 1, 64), 1, "float16", "float32", [2, 1], 0),
+    ((4, 4, 64), 16, "float16", "float32", [16, 9], 40),  # (16 rows: one)
+    ((17, 1, 128), 32, "float16", "float32", [1], 300),
+    ((6, 2, 96), 8, "float16", "float32", [11, 12], 33),
+]
+
+
+@pytest.mark.parametrize("case", MANY_ROWS, ids=str)
+def test_decode_of_many_rows(gpu, lib, case):
+    import torch
+    layout, page, dtype, out, news, window = case
+    dtype, out = getattr(torch, dtype), getattr(torch, out)
+    lengths = [(news[i % len(news)], n) for i, n in enumerate(LENGTHS + [1500, 4001])]
+    bound = -(-(1 << 17) // len(lengths) // layout[1])
+    bound = max(bound, 4001 + max(news))
+    k, v, table, q_start, kv_len, q = make(torch, layout, page, dtype, lengths, 31, unmapped=[(18, 700 // page)],
+                                           width=-(-bound // page) + 1)
+    cache, batch = build(torch, layout, k, v, table, q_start, kv_len, max(news), bound)
+    ref = reference(torch, k, v, table, lengths, q, window, layout[2] ** -0.5)
+    y = torch.full(q.shape, float("nan"), dtype=out, device="cuda")
+    first = None
+    for _ in range(3):
+        check(torch, cache.attend_decode(batch, q, out=y.fill_(float("nan")), window=window), ref, dtype, False)
+        first = y.clone() if first is None else first
+        assert torch.equal(first, y)
+    # what no row of a sequence sees, and what only its last row sees
+    if window == 0 and max(news) > 1:
+        s = max(i for i, (n, o) in enumerate(lengths) if n > 1)
+        n, o = lengths[s]
+        last = o + n - 1
+        v[int(table[s, last // page]), :, last % page] = float("inf")
+        y = cache.attend_decode(batch, q, out=torch.empty_like(q, dtype=torch.float32))
+        row = int(q_start[s + 1]) - 1
+        keep = [r for r in range(q.shape[0]) if r != row]
+        check(torch, y[keep], [t[keep] for t in ref], dtype, False)
+        assert not torch.isfinite(y[row]).any()
