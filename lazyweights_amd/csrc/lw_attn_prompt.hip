@@ -97,12 +97,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const AttnArgs a) {
   const int wlo = past + by_group(min(r0 + 32 * w, R - 1)), whi = past + by_group(min(r0 + 32 * w + 31, R - 1));
   const bool full = r0 + 32 * w + 32 <= R, empty = r0 + 32 * w >= R;
   const u32x4 flip = (u32x4)(uint32_t)__builtin_amdgcn_readfirstlane(a.q_flip);
+  // (past the last row: that row's q, for which nothing is seen or written; a branch would have each load waited for by itself)
+  const int q_row = min(row, R - 1), q_tok = by_group(q_row);
+  const uint16_t* q_from = a.q + (int64_t)(sq.row0 + q_tok) * a.ldq + (int64_t)(kvh * a.group + q_row - q_tok * a.group) * D + 8 * g;
   u32x4 qf[2 * C];
 #pragma unroll
-  for (int i = 0; i < 2 * C; ++i)
-    qf[i] = row < R ? *reinterpret_cast<const u32x4*>(a.q + (int64_t)(sq.row0 + tok) * a.ldq + (int64_t)head * D + 16 * i + 8 * g) ^
-                          flip
-                    : (u32x4)0;
+  for (int i = 0; i < 2 * C; ++i) qf[i] = *reinterpret_cast<const u32x4*>(q_from + 16 * i) ^ flip;
 
   const int lrow = ((lane & 15) - 4 * (lane >> 4)) & 15;  // the row of its block that this lane copies
   const int32_t* table = c.table + s * c.tstride;
