@@ -418,8 +418,8 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 // a few tens of rows are bound by memory and the matrix cores are used for their layout (an item of 4 rows fills a quarter of a
 // tile's columns, the matrix cores busy 5 % of the time). A wave has a tile's 32 keys and values in flight to registers (16 KB at D = 128)
 // while it works on the one before; V goes through LDS, its own, for the transposed reads. Times (us, and of what bytes):
-// 64 sequences of 500-16000 keys, 8 heads of 128: 196 (1.05 GB: 5.4 TB/s, of the 6.7 that a stream of reads reaches); one of
-// 131071: 97 (537 MB: 5.5); 4 x 5 tokens of 32 heads of 96 over 301-5003: 29 (101 MB); one of 778: 13. What separates the
+// 64 sequences of 500-16000 keys, 8 heads of 128: 194 (1.05 GB: 5.4 TB/s, of the 6.7 that a stream of reads reaches); one of
+// 131071: 97 (537 MB: 5.5); 4 x 5 tokens of 32 heads of 96 over 301-5003: 28 (101 MB); one of 778: 12.7. What separates the
 // first two from that stream are mostly the launch's ends, and the others are little else: the XCDs start up to 4 us after one
 // another, then come the lengths, a page number, its keys, and at the end the join of runs, each waiting for the one before.
 template <int D, bool BF, int RT, int NW>

@@ -58,10 +58,10 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int tile) {
 // Per 64 keys and 32 rows a wave has 32 matrix instructions of 32 cycles (D = 128, one-part weights) and some 170 vector
 // instructions (a score's scaling, exponential, conversion; its share of maximum and sum), 32 of them exponentials at a
 // quarter of the rate: 1024 cycles beside about 1100, which the SIMD's two waves run against each other. 15999 tokens of
-// 32 heads of 128, bf16: 2.10 TFLOP in 2070 us, 1013 TFLOP/s (a library product of 16384 in each direction reaches 1338);
+// 32 heads of 128, bf16: 2.10 TFLOP in 1960 us, 1070 TFLOP/s (a library product of 16384 in each direction reaches 1338);
 // the matrix cores are busy half of the cycles, and the card holds its clock at 1.75 to 1.95 of 2.4 GHz meanwhile. fp32
 // outputs take two- or three-part weights, half as many or as many matrix instructions more: 9 ragged prompts of 17-2500
-// tokens, 32 heads of 96, 55 GFLOP (83 with both parts) in 129 us. Row tiles with the most keys first over all sequences (they
+// tokens, 32 heads of 96, 55 GFLOP (83 with both parts) in 127 us. Row tiles with the most keys first over all sequences (they
 // are so within each) lost 5 to 14 %: neighbouring tiles then no longer share keys in an XCD's L2, and each block has to
 // find its tile.
 //
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const AttnArgs a) {
       }
     };
     // the same with four buffers of V, and the tiles before and after those that its rows see in loops of their own: a branch
-    // around the products has their sums moved from register to register (15999 tokens 2070 us against 2140; of two buffers
+    // around the products has their sums moved from register to register (15999 tokens 2070 us against 2140 then; of two buffers
     // the branch is up to 3 % faster)
     auto run4 = [&] {
       auto copies = [&](int t, int end) {
