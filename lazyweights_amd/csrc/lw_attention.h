@@ -62,7 +62,9 @@ struct AttnArgs {
   float* part;
   uint32_t* count;
   int row_blocks, blocks_log2, most_keys, whole;
-  int splits;  // the prompt kernel's: blocks that share the keys of a row tile, their sums in `part`
+  // the prompt kernel's
+  int splits;    // blocks that share the keys of a row tile, their sums in `part`
+  int most_run;  // about as many keys as one block goes through, at most
 };
 
 // How the decode kernel divides a batch: row_tiles tiles of 16 (token, head) rows per item, row_blocks items for a
@@ -77,7 +79,8 @@ DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_
 
 // The prompt kernel's row tiles of 128 (token, head) rows of a key-value head, and into how many blocks the keys of each are shared
 // out, with a workspace of `slots` slots of prompt_slot_bytes() each (kPromptSlots are of use).
-constexpr int kPromptSlots = 512;
+// Runs of more than kLongRun keys are summed with more care for fp32 outputs.
+constexpr int kPromptSlots = 512, kLongRun = 16384;
 int64_t prompt_items(int seqs, int kv_heads, int group, int tokens);
 size_t prompt_slot_bytes(int head_dim);
 int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots);

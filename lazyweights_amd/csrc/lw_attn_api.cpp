@@ -101,6 +101,7 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   a.count = nullptr;
   a.row_blocks = a.blocks_log2 = a.most_keys = a.whole = 0;
   a.splits = 1;
+  a.most_run = 0;
   return 0;
 }
 
@@ -201,6 +202,8 @@ int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
       a.splits = lw::prompt_splits(batch->seqs, cache->kv_heads, a.group, batch->tokens, batch->max_kv,
                                    bytes / (long long)lw::prompt_slot_bytes(cache->head_dim));
   }
+  const int most_kv = a.window > 0 ? std::min(batch->max_kv, a.window) : batch->max_kv;
+  a.most_run = most_kv / a.splits;
   return launched(fn, lw::launch_attn_prompt(a, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
 }
 

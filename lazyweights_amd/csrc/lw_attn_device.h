@@ -107,6 +107,13 @@ __device__ __forceinline__ int last_at_most(int n, int x, F first) {
   return lo;
 }
 
+// sum += x, with what rounding has added to the sum so far taken off x first (W. Kahan, 1965)
+__device__ __forceinline__ void add_exactly(float& sum, float& lost, float x) {
+  const float y = x - lost, t = sum + y;
+  lost = (t - sum) - y;
+  sum = t;
+}
+
 // a sequence's rows and keys, whatever the arrays hold: rows lie in [0, tokens), keys in the page table
 struct Seq {
   int row0, rows, len;
