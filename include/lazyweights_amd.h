@@ -266,9 +266,10 @@ int lw_kv_append(const lw_kv_cache* cache, const lw_batch* batch, int heads, con
  * zeros; keys and values that a row does not see never reach it, whatever they hold. q [tokens][heads][head_dim] of
  * the cache's type (row stride ldq), out of out_type (row stride ldo); alignment as lw_kv_append's. Scores, weights'
  * sums and outputs are accumulated in fp32. lw_attn_decode is for max_new <= 16 (one new token per sequence, or a few
- * that are verified together): the keys are split over the GPU and joined in order, the weights keep 22 bits or more.
- * lw_attn_prompt takes any number; with a 16-bit out its weights are rounded to the cache's type, with LW_F32 they keep
- * 22 bits or more. Both give the same bits on every call. Asynchronous on `stream`, allocate nothing, can be captured.
+ * that are verified together): the keys are split over the GPU and joined in order, the weights keep 22 bits (fp16
+ * cache; what is below 2^-40 of the row's largest weight is lost) or 24 (bf16). lw_attn_prompt takes any number; with
+ * LW_F32 its weights keep as many (2^-36 there), with a 16-bit out they are rounded to the cache's type (11 bits and 2^-36, or 8),
+ * about as much as the output's own rounding. Both give the same bits on every call. Asynchronous on `stream`, allocate nothing, can be captured.
  * Return 0 or -1. */
 int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, long long ldq, void* out,
                    int out_type, long long ldo, float scale, int window, void* stream);

@@ -88,6 +88,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
                                             int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0, int T,
                                             uint32_t run, int lane, int w, int n, int g) {
   constexpr int C = D / 32, DT = D / 16, NP = BF ? 3 : 2;
+  constexpr float LIFT = lift<BF>(0);
   const KvView& c = a.c;
   const Divisor by_group = a.by_group;
   const int R = sq.rows * a.group, r0 = rb * RT * 16;
@@ -206,7 +207,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
 #pragma unroll
         for (int e = 1; e < 8; ++e) mx = fmaxf(mx, p[r][e]);
         mx = fmaxf(max32(max16(mx)), m[r]);
-        const float base = mx == -INFINITY ? 0.f : mx, down = pow2(m[r] - base);
+        const float top = mx == -INFINITY ? 0.f : mx, down = pow2(m[r] - top), base = top - LIFT;
         m[r] = mx;
         float sum = 0.f;
 #pragma unroll

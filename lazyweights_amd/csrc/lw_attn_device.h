@@ -160,6 +160,16 @@ __device__ __forceinline__ f2v get2(const float* p) {
   return (f2v){__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32))};
 }
 
+// Weights are 2^(score - m + lift), m the row's largest score or less by `ahead` at most; numerators and sums carry the same
+// factor. The least step of fp16 is 2^-24, in a second part too, so what rounding takes from a weight is up to 2^-25 of the unit.
+// Lifted so that the largest is 2^15 (65504 is the last number), or 2^(15 - ahead) at least, that is 2^-40, or 2^(ahead - 40), of
+// the row's largest weight; not lifted, a weight e^-17.4 of the largest would be lost whole, while the row's sum counts it.
+// bf16 has the range of fp32.
+template <bool BF>
+constexpr float lift(float ahead) {
+  return BF ? 0.f : 15.f - ahead;
+}
+
 // weights p as the operand of the second product, in NP 16-bit parts that add up to p (two of fp16: 22 bits, three of
 // bf16: 24; one: rounded)
 template <bool BF, int NP>
