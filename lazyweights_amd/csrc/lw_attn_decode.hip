@@ -445,10 +445,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_decode(const AttnArgs a) {
     if (T) decode_item<D, BF, RT, NW>(a, smem, ml, pcare, &last_block, s, sq, hb - rb * kv_heads, rb, first_key(sq), 0, T, 0, T, T, lane, w, n, g);
     return;
   }
-  // the sequences are held 64 at a time, one per lane, with their tiles and those up to theirs
-  Seq mine;
-  uint32_t own, upto;
-  int held;
+  // the sequences are held 64 at a time, one per lane, with their tiles and those up to theirs (none yet: of two or three times 64,
+  // a block's last waves hold none before the run's first)
+  Seq mine = {0, 0, 0};
+  uint32_t own = 0, upto = 0;
+  int held = -1;
   auto hold = [&](int chunk) __attribute__((always_inline)) {
     held = chunk;
     mine = {0, 0, 0};
