@@ -84,6 +84,9 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
       ldo < (long long)heads * cache->head_dim)
     return refuse(fn, "q and out must be aligned to 16 bytes, with row strides of multiples of 8 that hold their heads");
   a.c = view(*cache, *batch);
+  // (where a page is not there the kernels load the first page's keys instead and leave them out: of no pages there is no first, so
+  // no sequence has keys, and all rows are zeros)
+  if (cache->pages == 0) a.c.table_pages = 0;
   a.q = static_cast<const uint16_t*>(q);
   a.out = out;
   a.ldq = ldq;
