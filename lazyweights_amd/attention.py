@@ -9,8 +9,11 @@ lw_attn_prompt).
 
 The tensors of a batch (q_start, kv_len, page_table) are read on the GPU when a call runs: a program that writes the next
 step's lengths and pages into them keeps the batch, and can capture its calls, as long as max_new and max_kv bound them.
-Calls go to torch's current stream unless `stream` (a hipStream_t as an integer) is given. Bad arguments raise ValueError;
-a call that the library refuses raises RuntimeError with lw_last_error().
+Calls go to torch's current stream unless `stream` (a hipStream_t as an integer) is given. Then what a call returns belongs to
+that stream, and the memory of what it reads is not given to others before the call is done (torch's record_stream: a stream
+of the caller's own has to outlive these tensors); that the given stream waits for what made the inputs (a Batch fills its
+workspace on the stream that is current when it is made) is the caller's part, as with all of torch. Bad arguments raise
+ValueError; a call that the library refuses raises RuntimeError with lw_last_error().
 """
 import ctypes
 
@@ -116,6 +119,25 @@ class KvCache:
                              "wanted, not %s" % (what, heads, dim, tuple(shape)))
         return x.data_ptr(), stride[0] if shape[0] > 1 else heads * dim
 
+    def _other(self, stream):
+        """torch's stream of the handle `stream`; None if that is the current one (or none is given)."""
+        if stream is None or stream == self._current(self.index):
+            return None
+        return torch.cuda.ExternalStream(stream, self.index) if stream else torch.cuda.default_stream(self.index)
+
+    def _empty(self, shape, other):
+        """A new tensor of the cache's type, of the memory of the stream that is going to write it."""
+        if other is None:
+            return torch.empty(shape, dtype=self.k.dtype, device=self.k.device)
+        with torch.cuda.stream(other):
+            return torch.empty(shape, dtype=self.k.dtype, device=self.k.device)
+
+    def _used(self, other, batch, *tensors):
+        """Keeps the memory of a call's tensors from others until the stream `other` has done the call."""
+        for t in (self.k, self.v, batch.workspace) + batch.tensors + tensors:
+            if t is not None:
+                t.record_stream(other)
+
     def append(self, batch, q, k, v, cos=None, sin=None, q_out=None, neighbours=False, stream=None):
         """Appends the rows k, v [tokens, kv_heads, head_dim] of the batch's new tokens, k rotated by its position, and
         returns q [tokens, heads, head_dim], rotated alike, in the cache's type (q may be None: keys and values only).
@@ -128,11 +150,12 @@ class KvCache:
             raise ValueError("q, k and v must have one of the types float32, float16, bfloat16 and the same number of rows")
         kp, ldk = self._rows("k", k, self.kv_heads)
         vp, ldv = self._rows("v", v, self.kv_heads)
+        other = self._other(stream)
         qp, ldq, op, ldo = None, 0, None, 0
         if q is not None:
             qp, ldq = self._rows("q", q, heads)
             if q_out is None:
-                q_out = torch.empty((n, heads, self.head_dim), dtype=self.k.dtype, device=self.k.device)
+                q_out = self._empty((n, heads, self.head_dim), other)
             elif q_out.dtype != self.k.dtype or q_out.shape[0] != n:
                 raise ValueError("q_out must have the cache's type and q's rows")
             op, ldo = self._rows("q_out", q_out, heads)
@@ -147,6 +170,8 @@ class KvCache:
         if self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
                                  1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream) != 0:
             raise RuntimeError(last_error())
+        if other is not None:
+            self._used(other, batch, q, k, v, cos, sin, q_out)
         return q_out
 
     def _attend(self, call, batch, q, out, scale, window, stream):
@@ -154,8 +179,9 @@ class KvCache:
         if q.dtype != self.k.dtype:
             raise ValueError("q must have the cache's type")
         qp, ldq = self._rows("q", q, heads)
+        other = self._other(stream)
         if out is None:
-            out = torch.empty(q.shape, dtype=self.k.dtype, device=self.k.device)
+            out = self._empty(q.shape, other)
         kind = self.types.get(out.dtype)
         if kind is None or out.shape[0] != q.shape[0]:
             raise ValueError("out must be float32, float16 or bfloat16, with q's rows")
@@ -164,6 +190,8 @@ class KvCache:
         if call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
                 window, self._current(self.index) if stream is None else stream) != 0:
             raise RuntimeError(last_error())
+        if other is not None:
+            self._used(other, batch, q, out)
         return out
 
     def attend_decode(self, batch, q, out=None, scale=None, window=0, stream=None):
