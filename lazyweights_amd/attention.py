@@ -55,7 +55,9 @@ class Batch:
     """`seqs` sequences whose new tokens are the rows of a call: q_start int32 [seqs + 1], kv_len int32 [seqs] (the lengths
     with the new tokens), page_table int32 [seqs, pages], all on the cache's GPU. max_new and max_kv bound every
     sequence's new tokens and length. A call's tensors may have more rows than q_start names; those are left alone. Holds
-    the workspace of attend_decode and attend_prompt, so calls with one batch must not overlap."""
+    the workspace of attend_decode and attend_prompt, so calls with one batch must not overlap. It serves every cache on its
+    device whose page tables are the same (all layers of a model); with max_new <= 16 attention is for caches of as many
+    key-value heads as the one it was made for, since the workspace's counters are laid out by them."""
 
     def __init__(self, cache, heads, q_start, kv_len, page_table, max_new, max_kv):
         seqs = kv_len.shape[0]
@@ -69,6 +71,7 @@ class Batch:
                 raise ValueError("q_start, kv_len and the rows of page_table must be contiguous")
         self.heads, self.max_new, self.max_kv = int(heads), int(max_new), int(max_kv)
         self.tensors = (q_start, kv_len, page_table)  # kept alive
+        self.index, self.kv_heads = cache.index, cache.kv_heads
         self.c = _Batch(seqs, 0, self.max_new, self.max_kv, q_start.data_ptr(), kv_len.data_ptr(),
                         page_table.data_ptr(), page_table.stride(0) if seqs > 1 else page_table.shape[1],
                         page_table.shape[1], 0, None, 0)
@@ -144,6 +147,8 @@ class KvCache:
         q, k and v have one type (float32, float16 or bfloat16); rows may be views into a joined projection. cos, sin
         float32 [positions, rot / 2] rotate the first rot elements of a head in pairs (j, j + rot / 2), or (2 j, 2 j + 1)
         with `neighbours`; without them nothing is rotated."""
+        if batch.index != self.index:
+            raise ValueError("the batch is on another device than the cache")
         heads, n = batch.heads, k.shape[0]
         kind = self.types.get(k.dtype)
         if kind is None or v.dtype != k.dtype or v.shape[0] != n or (q is not None and (q.dtype != k.dtype or q.shape[0] != n)):
@@ -176,6 +181,10 @@ class KvCache:
 
     def _attend(self, call, batch, q, out, scale, window, stream):
         heads = batch.heads
+        if batch.index != self.index:
+            raise ValueError("the batch is on another device than the cache")
+        if batch.kv_heads != self.kv_heads and batch.max_new <= 16:
+            raise ValueError("the batch is for caches of %d key-value heads, not %d" % (batch.kv_heads, self.kv_heads))
         if q.dtype != self.k.dtype:
             raise ValueError("q must have the cache's type")
         qp, ldq = self._rows("q", q, heads)
