@@ -213,7 +213,8 @@ enum { LW_F32 = 0, LW_F16 = 1, LW_BF16 = 2 };
 
 /* A caller-owned cache on the GPU: row r of page p of key-value head h starts at k (v) + p * page_stride + h * head_stride +
  * r * row_stride elements of `type` (LW_F16 or LW_BF16) and holds head_dim contiguous elements (64, 96 or 128). Pages of
- * page_size rows, a power of two up to 65536; strides are multiples of 8 elements, k and v aligned to 16 bytes. */
+ * page_size rows, a power of two up to 65536; strides are multiples of 8 elements, k and v aligned to 16 bytes. Calls are
+ * made with the cache's GPU as the calling thread's current one, where `stream` is. */
 typedef struct lw_kv_cache {
   void* k;
   void* v;

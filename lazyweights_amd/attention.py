@@ -51,6 +51,11 @@ def _current_stream():
     return raw or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _current_device():
+    """A function: the index of torch's current device."""
+    return getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 class Batch:
     """`seqs` sequences whose new tokens are the rows of a call: q_start int32 [seqs + 1], kv_len int32 [seqs] (the lengths
     with the new tokens), page_table int32 [seqs, pages], all on the cache's GPU. max_new and max_kv bound every
@@ -98,7 +103,7 @@ class KvCache:
         self.lib, self.k, self.v = load_library(), k, v
         self.kv_heads, self.head_dim = k.shape[1], k.shape[3]
         self.types, self.index = types, k.get_device()
-        self._current = _current_stream()
+        self._current, self._device = _current_stream(), _current_device()
         self.c = _Cache(k.data_ptr(), v.data_ptr(), k.shape[0], k.stride(0), k.stride(1), k.stride(2), k.shape[2],
                         k.shape[1], k.shape[3], types[k.dtype])
         self.ptr = ctypes.addressof(self.c)
@@ -121,6 +126,17 @@ class KvCache:
             raise ValueError("%s: [tokens, %d, %d] (or the two last joined) with contiguous rows on the cache's device is "
                              "wanted, not %s" % (what, heads, dim, tuple(shape)))
         return x.data_ptr(), stride[0] if shape[0] > 1 else heads * dim
+
+    def _launch(self, call, *args):
+        """The library's call, with the cache's device as the current one: launches go to the current device, also on a default
+        stream, whose handle is the same for all of them."""
+        if self._device() == self.index:
+            done = call(self.ptr, *args)
+        else:
+            with torch.cuda.device(self.index):
+                done = call(self.ptr, *args)
+        if done != 0:
+            raise RuntimeError(last_error())
 
     def _other(self, stream):
         """torch's stream of the handle `stream`; None if that is the current one (or none is given)."""
@@ -172,9 +188,8 @@ class KvCache:
                 raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
             cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
         batch.c.tokens = n
-        if self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
-                                 1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream) != 0:
-            raise RuntimeError(last_error())
+        self._launch(self.lib.lw_kv_append, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
+                     1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream)
         if other is not None:
             self._used(other, batch, q, k, v, cos, sin, q_out)
         return q_out
@@ -196,9 +211,8 @@ class KvCache:
             raise ValueError("out must be float32, float16 or bfloat16, with q's rows")
         op, ldo = self._rows("out", out, heads)
         batch.c.tokens = q.shape[0]
-        if call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
-                window, self._current(self.index) if stream is None else stream) != 0:
-            raise RuntimeError(last_error())
+        self._launch(call, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
+                     window, self._current(self.index) if stream is None else stream)
         if other is not None:
             self._used(other, batch, q, out)
         return out

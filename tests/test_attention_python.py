@@ -26,7 +26,7 @@ def cache(lib, kv_heads=8, head_dim=64, pages=4, page=16):
     c.lib, c.k, c.v = lib, *(torch.zeros((pages, kv_heads, page, head_dim), dtype=torch.float16) for _ in range(2))
     c.kv_heads, c.head_dim, c.index = kv_heads, head_dim, c.k.get_device()
     c.types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    c._current = lambda index: 0
+    c._current, c._device = lambda index: 0, lambda: c.index
     c.c = _Cache(c.k.data_ptr(), c.v.data_ptr(), pages, c.k.stride(0), c.k.stride(1), c.k.stride(2), page, kv_heads, head_dim, 1)
     c.ptr = ctypes.addressof(c.c)
     return c
@@ -69,3 +69,34 @@ def test_a_batch_of_another_device(lib):
         with pytest.raises(ValueError, match="device"):
             call()
     assert not calls.made
+
+
+def test_calls_are_made_with_the_caches_device_current(lib, monkeypatch):
+    """Default streams of all devices have the same handle: the launch goes to the current device, which must be the cache's."""
+    device = [3]
+    calls = Calls(lib)
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, device[0] = device[0], self.index
+
+        def __exit__(self, *exc):
+            device[0] = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    seen = []
+    calls.lw_kv_append = calls.lw_attn_decode = calls.lw_attn_prompt = lambda *args: seen.append(device[0]) or 0
+    c = cache(calls)
+    c._device = lambda: device[0]
+    b = batch(c)
+    k = torch.zeros((64, 8, 64))
+    for device[0] in (3, c.index):
+        outside = device[0]
+        c.append(b, None, k, k)
+        c.attend_decode(b, q_of(c))
+        c.attend_prompt(b, q_of(c))
+        assert device[0] == outside
+    assert seen == 6 * [c.index]
