@@ -127,20 +127,9 @@ class KvCache:
                              "wanted, not %s" % (what, heads, dim, tuple(shape)))
         return x.data_ptr(), stride[0] if shape[0] > 1 else heads * dim
 
-    def _launch(self, call, *args):
-        """The library's call, with the cache's device as the current one: launches go to the current device, also on a default
-        stream, whose handle is the same for all of them."""
-        if self._device() == self.index:
-            done = call(self.ptr, *args)
-        else:
-            with torch.cuda.device(self.index):
-                done = call(self.ptr, *args)
-        if done != 0:
-            raise RuntimeError(last_error())
-
     def _other(self, stream):
-        """torch's stream of the handle `stream`; None if that is the current one (or none is given)."""
-        if stream is None or stream == self._current(self.index):
+        """torch's stream of the handle `stream`; None if that is the current one."""
+        if stream == self._current(self.index):
             return None
         return torch.cuda.ExternalStream(stream, self.index) if stream else torch.cuda.default_stream(self.index)
 
@@ -163,6 +152,9 @@ class KvCache:
         q, k and v have one type (float32, float16 or bfloat16); rows may be views into a joined projection. cos, sin
         float32 [positions, rot / 2] rotate the first rot elements of a head in pairs (j, j + rot / 2), or (2 j, 2 j + 1)
         with `neighbours`; without them nothing is rotated."""
+        if self._device() != self.index:  # launches go to the current device
+            with torch.cuda.device(self.index):
+                return self.append(batch, q, k, v, cos, sin, q_out, neighbours, stream)
         if batch.index != self.index:
             raise ValueError("the batch is on another device than the cache")
         heads, n = batch.heads, k.shape[0]
@@ -171,7 +163,7 @@ class KvCache:
             raise ValueError("q, k and v must have one of the types float32, float16, bfloat16 and the same number of rows")
         kp, ldk = self._rows("k", k, self.kv_heads)
         vp, ldv = self._rows("v", v, self.kv_heads)
-        other = self._other(stream)
+        other = None if stream is None else self._other(stream)
         qp, ldq, op, ldo = None, 0, None, 0
         if q is not None:
             qp, ldq = self._rows("q", q, heads)
@@ -188,13 +180,17 @@ class KvCache:
                 raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
             cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
         batch.c.tokens = n
-        self._launch(self.lib.lw_kv_append, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
-                     1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream)
+        if self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
+                                 1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream) != 0:
+            raise RuntimeError(last_error())
         if other is not None:
             self._used(other, batch, q, k, v, cos, sin, q_out)
         return q_out
 
     def _attend(self, call, batch, q, out, scale, window, stream):
+        if self._device() != self.index:  # launches go to the current device
+            with torch.cuda.device(self.index):
+                return self._attend(call, batch, q, out, scale, window, stream)
         heads = batch.heads
         if batch.index != self.index:
             raise ValueError("the batch is on another device than the cache")
@@ -203,7 +199,7 @@ class KvCache:
         if q.dtype != self.k.dtype:
             raise ValueError("q must have the cache's type")
         qp, ldq = self._rows("q", q, heads)
-        other = self._other(stream)
+        other = None if stream is None else self._other(stream)
         if out is None:
             out = self._empty(q.shape, other)
         kind = self.types.get(out.dtype)
@@ -211,8 +207,9 @@ class KvCache:
             raise ValueError("out must be float32, float16 or bfloat16, with q's rows")
         op, ldo = self._rows("out", out, heads)
         batch.c.tokens = q.shape[0]
-        self._launch(call, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
-                     window, self._current(self.index) if stream is None else stream)
+        if call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
+                window, self._current(self.index) if stream is None else stream) != 0:
+            raise RuntimeError(last_error())
         if other is not None:
             self._used(other, batch, q, out)
         return out
