@@ -75,6 +75,8 @@ class Batch:
             if t.numel() and t.stride(-1) != 1:
                 raise ValueError("q_start, kv_len and the rows of page_table must be contiguous")
         self.heads, self.max_new, self.max_kv = int(heads), int(max_new), int(max_kv)
+        if not all(-1 << 31 <= n < 1 << 31 for n in (self.heads, self.max_new, self.max_kv)):
+            raise ValueError("heads, max_new and max_kv must be numbers of 32 bits")  # (others would be cut to that)
         self.tensors = (q_start, kv_len, page_table)  # kept alive
         self.index, self.kv_heads = cache.index, cache.kv_heads
         self.c = _Batch(seqs, 0, self.max_new, self.max_kv, q_start.data_ptr(), kv_len.data_ptr(),
@@ -178,7 +180,7 @@ class KvCache:
                     or cos.shape != sin.shape or cos.get_device() != self.index or sin.get_device() != self.index
                     or not cos.is_contiguous() or not sin.is_contiguous()):
                 raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
-            cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1]
+            cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), min(cos.shape[0], (1 << 31) - 1), 2 * cos.shape[1]
         batch.c.tokens = n
         if self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
                                  1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream) != 0:
@@ -196,6 +198,8 @@ class KvCache:
             raise ValueError("the batch is on another device than the cache")
         if batch.kv_heads != self.kv_heads and batch.max_new <= 16:
             raise ValueError("the batch is for caches of %d key-value heads, not %d" % (batch.kv_heads, self.kv_heads))
+        if not 0 <= window < 1 << 31:  # (32 bits in the call: no position is that far back)
+            window = (1 << 31) - 1 if window > 0 else -1
         if q.dtype != self.k.dtype:
             raise ValueError("q must have the cache's type")
         qp, ldq = self._rows("q", q, heads)

@@ -100,3 +100,21 @@ def test_calls_are_made_with_the_caches_device_current(lib, monkeypatch):
         c.attend_prompt(b, q_of(c))
         assert device[0] == outside
     assert seen == 6 * [c.index]
+
+
+@pytest.mark.parametrize("big", [dict(heads=2 ** 32 + 32), dict(max_new=2 ** 32 + 1), dict(max_kv=2 ** 32 + 64),
+                                 dict(max_kv=-2 ** 32 + 64), dict(max_new=2 ** 31)], ids=str)
+def test_sizes_past_32_bits_are_refused(lib, big):
+    """They would be cut to their low 32 bits, which the library could find fine."""
+    with pytest.raises(ValueError):
+        batch(cache(Calls(lib)), **big)
+
+
+def test_windows_past_32_bits(lib):
+    """A window that no sequence can fill hides nothing; a negative one stays one, which the library refuses."""
+    calls = Calls(lib)
+    c = cache(calls)
+    b = batch(c)
+    for window in (5, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, -1, -2 ** 32 + 5):
+        c.attend_decode(b, q_of(c), window=window)
+    assert [args[-2] for args in calls.made] == [5, 2 ** 31 - 1, 2 ** 31 - 1, 2 ** 31 - 1, -1, -1]
