@@ -70,6 +70,8 @@ class Layer:
 class Sequences:
     """Lengths and pages of the sequences in a layer's cache."""
 
+    KEPT = 8  # batches
+
     def __init__(self, layer, count, most):
         page = layer.cache.k.shape[2]
         self.layer, self.page, self.most = layer, page, most
@@ -89,13 +91,19 @@ class Sequences:
         self.kv_len.copy_(torch.tensor(self.lengths, dtype=torch.int32))
 
     def batch(self, news):
-        """The batch in which every sequence has news[s] new tokens; one of a kind is kept."""
+        """The batch in which every sequence has news[s] new tokens; the last KEPT kinds of them are kept, each with its workspace
+        (steps of single tokens and drafts come again and again, prompts hardly ever in the same lengths; who captures a call keeps
+        its batch)."""
         self.grow(news)
         key = tuple(news)
-        if key not in self.steady:
+        batch = self.steady.pop(key, None)
+        if batch is None:
             starts = torch.tensor([0] + news, dtype=torch.int32).cumsum(0, dtype=torch.int32).cuda()
-            self.steady[key] = Batch(self.layer.cache, self.layer.heads, starts, self.kv_len, self.table, max(news), self.most)
-        return self.steady[key]
+            batch = Batch(self.layer.cache, self.layer.heads, starts, self.kv_len, self.table, max(news), self.most)
+        self.steady[key] = batch  # (the last one used at the end)
+        while len(self.steady) > self.KEPT:
+            del self.steady[next(iter(self.steady))]
+        return batch
 
 
 def main():
