@@ -255,7 +255,7 @@ long long lw_attn_workspace(const lw_kv_cache* cache, const lw_batch* batch, int
  * of the cache's type with row stride ldo. Pointers are aligned to 16 bytes, strides multiples of 8. cos, sin: fp32
  * [rope_rows][rot / 2], rope_rows >= max_kv, rot <= head_dim a multiple of 8: the first rot elements of a head are rotated, as
  * pairs (j, j + rot / 2), or with neighbours = 1 as pairs (2 j, 2 j + 1); the others are copied. rot = 0: no rotation. q
- * may be NULL (keys and values only). Rows of no sequence are left alone. Needs no workspace. Asynchronous on `stream`,
+ * may be NULL (keys and values only). Rows of no sequence, or before its first position, are left alone. Needs no workspace. Asynchronous on `stream`,
  * allocates nothing, can be captured. Returns 0 or -1. */
 int lw_kv_append(const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, const void* k, const void* v,
                  int x_type, long long ldq, long long ldk, long long ldv, const float* cos, const float* sin, int rot,
@@ -269,8 +269,8 @@ int lw_kv_append(const lw_kv_cache* cache, const lw_batch* batch, int heads, con
  * sums and outputs are accumulated in fp32. lw_attn_decode is for max_new <= 16 (one new token per sequence, or a few
  * that are verified together): the keys are split over the GPU and joined in order, the weights keep 22 bits (fp16
  * cache; what is below 2^-40 of the row's largest weight is lost) or 24 (bf16). lw_attn_prompt takes any number; with
- * LW_F32 its weights keep as many (2^-36 there), with a 16-bit out they are rounded to the cache's type (11 bits and 2^-36, or 8),
- * about as much as the output's own rounding. Both give the same bits on every call. Asynchronous on `stream`, allocate nothing, can be captured.
+ * LW_F32 its weights keep as many (2^-36 there), with a 16-bit out they are rounded to the cache's type (11 bits and 2^-36, or 8).
+ * Both give the same bits on every call. Asynchronous on `stream`, allocate nothing, can be captured.
  * Return 0 or -1. */
 int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, long long ldq, void* out,
                    int out_type, long long ldo, float scale, int window, void* stream);

@@ -446,6 +446,9 @@ __global__ __launch_bounds__(256) void k_attn_join(const AttnArgs a) {
   for (int j = 0; j < 4; ++j) store4(a.out_type, a.out, at + 8 * j, normal(o[j], l));
 }
 
+// Parts of the weights: all of them for fp32 outputs; one for 16-bit ones, whose own rounding is larger than what a row's average
+// shows of its weights' (1000 tokens after 9001, fp16: 2.2e-4 from 64 bits, 2.1e-4 where only the output is rounded; 15999 in bf16
+// 1.8e-3 and 1.7e-3). 9000 tokens of 32 heads of 128: fp16 756 us with one, 998 with two, bf16 653 with one, 1114 with three.
 template <int D, bool BF, int W>
 hipError_t prompt_w(const AttnArgs& a, int splits, hipStream_t s) {
   const dim3 grid((uint32_t)(((int64_t)a.c.tokens * a.group / (32 * W) + a.c.seqs) * a.c.kv_heads * splits));
