@@ -41,3 +41,41 @@ def test_prompt_sums_of_like_weights(gpu, lib, keys, dtype):
     bound = 2.0 ** -24 + 2.0 ** -21 + 2 * 2.0 ** -21 + 2.0 ** -20 + 4 * math.sqrt(keys / 16) * 2.0 ** -24
     print("worst relative error %.2g, bound %.2g" % (err, bound), flush=True)
     assert err <= bound
+
+
+@pytest.mark.parametrize("dtype", ("float16", "bfloat16"))
+@pytest.mark.parametrize("layout, new, old", [((32, 8, 128), 8200, 9000), ((32, 32, 96), 8200, 9000), ((32, 4, 64), 8200, 9000),
+                                              ((32, 8, 128), 900, 20000), ((7, 1, 64), 2000, 18000)], ids=str)
+def test_long_runs(gpu, lib, layout, new, old, dtype):
+    """Blocks of 8 and of 4 waves over more than 16384 keys, fp32 outputs, the last key's value not finite: some rows against 64 bits,
+    and the last, which alone sees that value. Bound as in the tests of any length: 2^-24 |out| + A (2^-21 + 2 2^-21 max_j scale
+    sum |q k_j| + 2^-20)."""
+    import torch
+    from lazyweights_amd import Batch, KvCache
+    heads, kv, dim = layout
+    kind, page, keys = getattr(torch, dtype), 64, new + old
+    pages, group = -(-keys // page), heads // kv
+    g = torch.Generator(device="cuda").manual_seed(42)
+    k = torch.randn((pages * page, kv, dim), generator=g, device="cuda").to(kind)
+    v = (torch.randn((pages * page, kv, dim), generator=g, device="cuda") + 0.25).to(kind)
+    q = (1.5 * torch.randn((new, heads, dim), generator=g, device="cuda")).to(kind)
+    v[keys - 1] = float("inf")
+    cache = KvCache(*(x.view(pages, page, kv, dim).transpose(1, 2).contiguous() for x in (k, v)))
+    batch = Batch(cache, heads, torch.tensor([0, new], dtype=torch.int32, device="cuda"),
+                  torch.tensor([keys], dtype=torch.int32, device="cuda"),
+                  torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous(), new, keys)
+    batch.c.workspace, batch.c.workspace_bytes = None, 0
+    y = cache.attend_prompt(batch, q, out=torch.full(q.shape, float("nan"), device="cuda"))
+    assert torch.isinf(y[-1]).all() and torch.isfinite(y[:-1]).all()
+    worst = 0.0
+    for row in [0, 1, 31, 32, 255, 256, new // 2, new - 300, new - 33, new - 2]:
+        n = old + row + 1
+        qq, kk, vv = q[row].double().view(kv, group, dim).cpu(), k[:n].double().cpu(), v[:n].double().cpu()
+        s = torch.einsum("hgd,jhd->hgj", qq, kk) * dim ** -0.5
+        p = torch.softmax(s, -1)
+        want, a = (torch.einsum("hgj,jhd->hgd", p, x).reshape(heads, dim) for x in (vv, vv.abs()))
+        most = (torch.einsum("hgd,jhd->hgj", qq.abs(), kk.abs()) * dim ** -0.5).amax(-1).reshape(heads, 1)
+        bound = 2.0 ** -24 * want.abs() + a * (2.0 ** -21 + 2 * 2.0 ** -21 * most + 2.0 ** -20)
+        worst = max(worst, ((y[row].double().cpu() - want).abs() / bound).max().item())
+    print("worst error / bound %.3f" % worst, flush=True)
+    assert worst <= 1
