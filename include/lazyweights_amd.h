@@ -277,6 +277,72 @@ int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
 int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, long long ldq, void* out,
                    int out_type, long long ldo, float scale, int window, void* stream);
 
+/* ── the same over a cache held in 8 bits, and the page tables of both (extensions: no counterpart in the reference) ── */
+
+/* A caller-owned cache on the GPU in 8 bits: row r of page p of key-value head h starts at byte p * page_stride + h * head_stride +
+ * r * row_stride of k (v) and holds head_dim (64, 96 or 128) numbers of 1 sign, 4 exponent and 3 mantissa bits (OCP e4m3: up to 448,
+ * no infinities); each block of 16 rows of a head has an exponent e in k_exp (v_exp)[p * exp_page_stride + h *
+ * exp_head_stride + r / 16], -48 to 48 (others are taken as the nearer of these): an element is its number times 2^e.
+ * Pages of page_size rows, a power of two from 16 to 65536; byte strides are multiples of 16, k and v aligned to 16 bytes. Calls
+ * are made with the cache's GPU as the calling thread's current one, where `stream` is. */
+typedef struct lw_kv8_cache {
+  void* k;
+  void* v;
+  int8_t* k_exp;
+  int8_t* v_exp;
+  int64_t pages, page_stride, head_stride, row_stride, exp_page_stride, exp_head_stride;
+  int32_t page_size, kv_heads, head_dim;
+  int32_t reserved; /* 0 */
+} lw_kv8_cache;
+
+/* lw_attn_workspace for lw_attn8_decode and lw_attn8_prompt. A batch's workspace serves the 8-bit calls or the 16-bit ones,
+ * not both (zero it in between). */
+long long lw_attn8_workspace(const lw_kv8_cache* cache, const lw_batch* batch, int heads);
+
+/* lw_kv_append into an 8-bit cache; q_out is of q_type (LW_F16 or LW_BF16). Rotated as there in fp32, each product and sum rounded
+ * for itself. A block's exponent is the least that holds the largest finite magnitude of its new rows (448 2^e at most, -48
+ * for zeros), or what it was where the block has rows from before the call's first new one and that is more; where it
+ * grows, those rows are rounded to it, once more. Numbers are rounded to nearest even; magnitudes past 448 2^48 are held as
+ * that, infinities as NaN. Rows behind a sequence's last are left alone. */
+int lw_kv8_append(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, const void* k, const void* v,
+                  int x_type, long long ldq, long long ldk, long long ldv, const float* cos, const float* sin, int rot,
+                  int rope_rows, int neighbours, void* q_out, int q_type, long long ldo, void* stream);
+
+/* lw_attn_decode and lw_attn_prompt over an 8-bit cache, q of q_type (LW_F16 or LW_BF16). Keys and values enter the
+ * products as the cache holds them; weights keep 22 bits (what is below 2^-40 of the largest product of a weight and its value's
+ * 2^e is lost; 2^-36 in prompts), 11 bits in lw_attn8_prompt with a 16-bit out. */
+int lw_attn8_decode(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, int q_type, long long ldq,
+                    void* out, int out_type, long long ldo, float scale, int window, void* stream);
+int lw_attn8_prompt(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, int q_type, long long ldq,
+                    void* out, int out_type, long long ldo, float scale, int window, void* stream);
+
+/* The pages of `seqs` sequences (up to 8192) and the pool of those that none has, on the GPU: position j of sequence s
+ * lies in row j % page_size of page table[s * table_stride + j / page_size]; free[0 .. left[0]) are the pool's pages, a
+ * stack, of `pages` at most. page_size is a power of two up to 65536. workspace: 4 bytes, zero before its first use; calls leave
+ * it zero, and calls that share one must not overlap. */
+typedef struct lw_pages {
+  int32_t* table;
+  int64_t table_stride;
+  int32_t table_pages, seqs, page_size, pages;
+  int32_t* free;    /* [pages] */
+  int32_t* kv_len;  /* [seqs] */
+  int32_t* left;    /* [2] */
+  int32_t* workspace;
+} lw_pages;
+
+/* A step of the sequences: s is cut to keep[s] tokens (keep NULL: to none of them) and grown by new_tokens[s]. Pages that it
+ * no longer needs go back, pages that it needs are taken and written to its row of the table; the i-th page taken (in the
+ * order of sequences and positions) is the i-th given back while there are any, then the last of the pool, and given pages that
+ * nobody takes are put on the pool's end in their order. kv_len_out[s] = min(keep, kv_len) + new; q_start [seqs + 1]: the
+ * sums of new_tokens before each sequence, the rows of a call (lw_batch); position[t], slot[t]: the position of row t and
+ * page * page_size + its row there, -1 where the page is outside [0, pages) (either may be NULL). left_out[0]: pages left; left_out[1]:
+ * 0, or what the call would have lacked, the sum of 1: pages, 2: room in the table, 4: rows. Then nothing is changed:
+ * the lengths and the pool are what they were, q_start is all 0. kv_len_out and left_out may be the pages' own. Table entries
+ * past a sequence's pages, and rows past the last, are left as they were. Negative numbers count as 0. Asynchronous on
+ * `stream`, allocates nothing, can be captured. Returns 0 or -1. */
+int lw_pages_advance(const lw_pages* pages, const int32_t* new_tokens, const int32_t* keep, int rows, int32_t* kv_len_out,
+                     int32_t* left_out, int32_t* q_start, int32_t* position, int64_t* slot, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

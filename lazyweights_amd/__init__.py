@@ -6,16 +6,17 @@ the skinny verify GEMM, behind the reference runtime's C-ABI (include/lazyweight
 from ._lib import LIB_PATH, last_error, load_library  # noqa: F401
 from .runtime import Runtime  # noqa: F401
 
-_ATTENTION = ("Batch", "KvCache")
+_TORCH = {"Batch": "attention", "KvCache": "attention", "KvCache8": "attention", "Pages": "pages"}
 
 
 def __getattr__(name):
-    """Batch and KvCache when they are first asked for: they need torch, which takes longer to import than all else here."""
-    if name in _ATTENTION:
-        from . import attention
-        return getattr(attention, name)
+    """Batch, KvCache, KvCache8 and Pages when they are first asked for: they need torch, which takes longer to import than all
+    else here."""
+    if name in _TORCH:
+        from importlib import import_module
+        return getattr(import_module("." + _TORCH[name], __name__), name)
     raise AttributeError("module %r has no attribute %r" % (__name__, name))
 
 
 def __dir__():
-    return sorted(set(globals()) | set(_ATTENTION))
+    return sorted(set(globals()) | set(_TORCH))

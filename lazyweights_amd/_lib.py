@@ -56,6 +56,12 @@ SIGNATURES = {
     "lw_kv_append": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _ll, _ll, _ll, _vp, _vp, _i, _i, _i, _vp, _ll, _vp]),
     "lw_attn_decode": (_i, [_vp, _vp, _i, _vp, _ll, _vp, _i, _ll, _c.c_float, _i, _vp]),
     "lw_attn_prompt": (_i, [_vp, _vp, _i, _vp, _ll, _vp, _i, _ll, _c.c_float, _i, _vp]),
+    # the same over a cache in 8 bits (lw_kv8_cache), and the page tables of both (lw_pages)
+    "lw_attn8_workspace": (_ll, [_vp, _vp, _i]),
+    "lw_kv8_append": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _ll, _ll, _ll, _vp, _vp, _i, _i, _i, _vp, _i, _ll, _vp]),
+    "lw_attn8_decode": (_i, [_vp, _vp, _i, _vp, _i, _ll, _vp, _i, _ll, _c.c_float, _i, _vp]),
+    "lw_attn8_prompt": (_i, [_vp, _vp, _i, _vp, _i, _ll, _vp, _i, _ll, _c.c_float, _i, _vp]),
+    "lw_pages_advance": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _LIB = None

@@ -1,8 +1,9 @@
 """Attention between a decoder layer's coded matrices, on torch tensors: a paged key-value cache, a batch of sequences over
 it, and the operators of include/lazyweights_amd.h that append to the cache and read it (lw_kv_append, lw_attn_decode,
-lw_attn_prompt).
+lw_attn_prompt; lw_kv8_append, lw_attn8_decode, lw_attn8_prompt over a cache held in 8 bits). lazyweights_amd/pages.py makes
+q_start, kv_len and page_table on the GPU.
 
-    cache = KvCache.empty(pages, kv_heads, page_size, head_dim)          # one per layer
+    cache = KvCache.empty(pages, kv_heads, page_size, head_dim)          # one per layer; or KvCache8, of half the size
     batch = Batch(cache, heads, q_start, kv_len, page_table, max_new, max_kv)  # one for all layers
     q16 = cache.append(batch, q, k, v, cos, sin)                         # q, k, v as the matrices give them, fp32
     y = cache.attend_decode(batch, q16)                                  # or attend_prompt, for more than 16 new tokens
@@ -56,13 +57,22 @@ def _current_device():
     return getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+class _Cache8(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("row_stride", ctypes.c_int64), ("exp_page_stride", ctypes.c_int64), ("exp_head_stride", ctypes.c_int64),
+                ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 class Batch:
     """`seqs` sequences whose new tokens are the rows of a call: q_start int32 [seqs + 1], kv_len int32 [seqs] (the lengths
     with the new tokens), page_table int32 [seqs, pages], all on the cache's GPU. max_new and max_kv bound every
     sequence's new tokens and length. A call's tensors may have more rows than q_start names; those are left alone. Holds
     the workspace of attend_decode and attend_prompt, so calls with one batch must not overlap. It serves every cache on its
     device whose page tables are the same (all layers of a model); with max_new <= 16 attention is for caches of as many
-    key-value heads as the one it was made for, since the workspace's counters are laid out by them."""
+    key-value heads as the one it was made for, and as it in 16 or in 8 bits, since the workspace's counters are laid out by
+    them."""
 
     def __init__(self, cache, heads, q_start, kv_len, page_table, max_new, max_kv):
         seqs = kv_len.shape[0]
@@ -78,12 +88,12 @@ class Batch:
         if not all(-1 << 31 <= n < 1 << 31 for n in (self.heads, self.max_new, self.max_kv)):
             raise ValueError("heads, max_new and max_kv must be numbers of 32 bits")  # (others would be cut to that)
         self.tensors = (q_start, kv_len, page_table)  # kept alive
-        self.index, self.kv_heads = cache.index, cache.kv_heads
+        self.index, self.kv_heads, self.eight = cache.index, cache.kv_heads, cache.eight
         self.c = _Batch(seqs, 0, self.max_new, self.max_kv, q_start.data_ptr(), kv_len.data_ptr(),
                         page_table.data_ptr(), page_table.stride(0) if seqs > 1 else page_table.shape[1],
                         page_table.shape[1], 0, None, 0)
         self.ptr = ctypes.addressof(self.c)
-        size = cache.lib.lw_attn_workspace(cache.ptr, self.ptr, self.heads)
+        size = cache._workspace_size(self)
         if size < 0:
             raise ValueError(last_error())
         self.workspace = torch.zeros(size, dtype=torch.uint8, device=cache.k.device)
@@ -93,6 +103,8 @@ class Batch:
 class KvCache:
     """Keys and values [pages, kv_heads, page_size, head_dim] of one layer, float16 or bfloat16 on the GPU, the caller's
     tensors or views of them with head_dim contiguous (k and v alike in their strides)."""
+
+    eight = False
 
     def __init__(self, k, v):
         types = _types()
@@ -117,6 +129,16 @@ class KvCache:
                 for _ in range(2))
         return cls(k, v)
 
+    def _workspace_size(self, batch):
+        return self.lib.lw_attn_workspace(self.ptr, batch.ptr, batch.heads)
+
+    def _memory(self):
+        return self.k, self.v
+
+    def _q_dtype(self, q_out):
+        """The type that q gets when it is appended, into q_out if that is given."""
+        return self.k.dtype
+
     def _rows(self, what, x, heads):
         """Address and row stride of x [tokens, heads, head_dim] or [tokens, heads * head_dim]."""
         shape, stride, dim = x.shape, x.stride(), self.head_dim
@@ -135,16 +157,16 @@ class KvCache:
             return None
         return torch.cuda.ExternalStream(stream, self.index) if stream else torch.cuda.default_stream(self.index)
 
-    def _empty(self, shape, other):
-        """A new tensor of the cache's type, of the memory of the stream that is going to write it."""
+    def _empty(self, shape, dtype, other):
+        """A new tensor of the memory of the stream that is going to write it."""
         if other is None:
-            return torch.empty(shape, dtype=self.k.dtype, device=self.k.device)
+            return torch.empty(shape, dtype=dtype, device=self.k.device)
         with torch.cuda.stream(other):
-            return torch.empty(shape, dtype=self.k.dtype, device=self.k.device)
+            return torch.empty(shape, dtype=dtype, device=self.k.device)
 
     def _used(self, other, batch, *tensors):
         """Keeps the memory of a call's tensors from others until the stream `other` has done the call."""
-        for t in (self.k, self.v, batch.workspace) + batch.tensors + tensors:
+        for t in self._memory() + (batch.workspace,) + batch.tensors + tensors:
             if t is not None:
                 t.record_stream(other)
 
@@ -166,12 +188,12 @@ class KvCache:
         kp, ldk = self._rows("k", k, self.kv_heads)
         vp, ldv = self._rows("v", v, self.kv_heads)
         other = None if stream is None else self._other(stream)
-        qp, ldq, op, ldo = None, 0, None, 0
+        qp, ldq, op, ldo, q_dtype = None, 0, None, 0, self._q_dtype(q_out)
         if q is not None:
             qp, ldq = self._rows("q", q, heads)
             if q_out is None:
-                q_out = self._empty((n, heads, self.head_dim), other)
-            elif q_out.dtype != self.k.dtype or q_out.shape[0] != n:
+                q_out = self._empty((n, heads, self.head_dim), q_dtype, other)
+            elif q_out.dtype != q_dtype or q_out.shape[0] != n:
                 raise ValueError("q_out must have the cache's type and q's rows")
             op, ldo = self._rows("q_out", q_out, heads)
         cp, sp, rot, rows = None, None, 0, 0
@@ -182,8 +204,13 @@ class KvCache:
                 raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
             cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), min(cos.shape[0], (1 << 31) - 1), 2 * cos.shape[1]
         batch.c.tokens = n
-        if self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
-                                 1 if neighbours else 0, op, ldo, self._current(self.index) if stream is None else stream) != 0:
+        args = (self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows, 1 if neighbours else 0, op)
+        where = self._current(self.index) if stream is None else stream
+        if self.eight:
+            rc = self.lib.lw_kv8_append(*args, self.types[q_dtype], ldo, where)
+        else:
+            rc = self.lib.lw_kv_append(*args, ldo, where)
+        if rc != 0:
             raise RuntimeError(last_error())
         if other is not None:
             self._used(other, batch, q, k, v, cos, sin, q_out)
@@ -198,21 +225,28 @@ class KvCache:
             raise ValueError("the batch is on another device than the cache")
         if batch.kv_heads != self.kv_heads and batch.max_new <= 16:
             raise ValueError("the batch is for caches of %d key-value heads, not %d" % (batch.kv_heads, self.kv_heads))
+        if batch.eight != self.eight and batch.max_new <= 16:
+            raise ValueError("the batch is for caches in %d bits" % (8 if batch.eight else 16))
         if not 0 <= window < 1 << 31:  # (32 bits in the call: no position is that far back)
             window = (1 << 31) - 1 if window > 0 else -1
-        if q.dtype != self.k.dtype:
+        if q.dtype != self._q_dtype(q):
             raise ValueError("q must have the cache's type")
         qp, ldq = self._rows("q", q, heads)
         other = None if stream is None else self._other(stream)
         if out is None:
-            out = self._empty(q.shape, other)
+            out = self._empty(q.shape, q.dtype, other)
         kind = self.types.get(out.dtype)
         if kind is None or out.shape[0] != q.shape[0]:
             raise ValueError("out must be float32, float16 or bfloat16, with q's rows")
         op, ldo = self._rows("out", out, heads)
         batch.c.tokens = q.shape[0]
-        if call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale,
-                window, self._current(self.index) if stream is None else stream) != 0:
+        args = (op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale, window,
+                self._current(self.index) if stream is None else stream)
+        if self.eight:
+            rc = call(self.ptr, batch.ptr, heads, qp, self.types[q.dtype], ldq, *args)
+        else:
+            rc = call(self.ptr, batch.ptr, heads, qp, ldq, *args)
+        if rc != 0:
             raise RuntimeError(last_error())
         if other is not None:
             self._used(other, batch, q, out)
@@ -228,3 +262,64 @@ class KvCache:
     def attend_prompt(self, batch, q, out=None, scale=None, window=0, stream=None):
         """attend_decode for any number of new tokens: whole prompts, or chunks of them after what is in the cache."""
         return self._attend(self.lib.lw_attn_prompt, batch, q, out, scale, window, stream)
+
+
+class KvCache8(KvCache):
+    """Keys and values of one layer in 8 bits: k and v float8_e4m3fn [pages, kv_heads, page_size, head_dim] on the GPU (as
+    KvCache's, page_size 16 at least), k_exp and v_exp int8 [pages, kv_heads, page_size / 16] with the last dimension
+    contiguous and alike in their strides: an element is its number times two to the exponent of its 16 rows' block. append
+    chooses the exponents (lw_kv8_append): the least that holds a block's new rows, and older rows of the block are rounded to a
+    larger one where it grows. q is float16 or bfloat16: append gives `q_dtype`, or the type of q_out. A Batch serves
+    caches of one kind only, of 8 or of 16 bits."""
+
+    eight = True
+
+    def __init__(self, k, v, k_exp, v_exp, q_dtype=None):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
+            raise ValueError("k and v must be [pages, kv_heads, page_size, head_dim], alike in type, device and strides")
+        if not k.is_cuda or k.dtype != torch.float8_e4m3fn:
+            raise ValueError("k and v must be float8_e4m3fn tensors on the GPU")
+        if k.stride(3) != 1:
+            raise ValueError("the elements of a head must be contiguous")
+        want = (k.shape[0], k.shape[1], k.shape[2] // 16)
+        if any(t.shape != want or t.dtype != torch.int8 or t.device != k.device for t in (k_exp, v_exp)):
+            raise ValueError("k_exp and v_exp must be int8 tensors [pages, kv_heads, page_size / 16] on the cache's device")
+        if k_exp.stride() != v_exp.stride() or (want[2] > 1 and k_exp.stride(2) != 1):
+            raise ValueError("k_exp and v_exp must be alike in their strides, a head's exponents contiguous")
+        self.lib, self.k, self.v, self.k_exp, self.v_exp = load_library(), k, v, k_exp, v_exp
+        self.kv_heads, self.head_dim = k.shape[1], k.shape[3]
+        self.types, self.index = _types(), k.get_device()
+        self.q_dtype = self._q_type(q_dtype or torch.float16)
+        self._current, self._device = _current_stream(), _current_device()
+        self.c = _Cache8(k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr(), k.shape[0], k.stride(0), k.stride(1),
+                         k.stride(2), k_exp.stride(0), k_exp.stride(1), k.shape[2], k.shape[1], k.shape[3], 0)
+        self.ptr = ctypes.addressof(self.c)
+
+    @classmethod
+    def empty(cls, pages, kv_heads, page_size, head_dim, q_dtype=None, device="cuda"):
+        """A new cache; its contents are whatever the memory held."""
+        k, v = (torch.empty((pages, kv_heads, page_size, head_dim), dtype=torch.float8_e4m3fn, device=device) for _ in range(2))
+        k_exp, v_exp = (torch.empty((pages, kv_heads, page_size // 16), dtype=torch.int8, device=device) for _ in range(2))
+        return cls(k, v, k_exp, v_exp, q_dtype)
+
+    def _workspace_size(self, batch):
+        return self.lib.lw_attn8_workspace(self.ptr, batch.ptr, batch.heads)
+
+    def _memory(self):
+        return self.k, self.v, self.k_exp, self.v_exp
+
+    def _q_type(self, dtype):
+        if self.types.get(dtype) not in (F16, BF16):
+            raise ValueError("q over an 8-bit cache is float16 or bfloat16")
+        return dtype
+
+    def _q_dtype(self, q_out):
+        return self.q_dtype if q_out is None else self._q_type(q_out.dtype)
+
+    def attend_decode(self, batch, q, out=None, scale=None, window=0, stream=None):
+        """KvCache.attend_decode, q float16 or bfloat16."""
+        return self._attend(self.lib.lw_attn8_decode, batch, q, out, scale, window, stream)
+
+    def attend_prompt(self, batch, q, out=None, scale=None, window=0, stream=None):
+        """KvCache.attend_prompt, q float16 or bfloat16."""
+        return self._attend(self.lib.lw_attn8_prompt, batch, q, out, scale, window, stream)

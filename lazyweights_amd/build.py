@@ -34,6 +34,8 @@ SOURCES = [
     ("lw_prefill.hip", "hip"),
     ("lw_attn_decode.hip", "hip"),
     ("lw_attn_prompt.hip", "hip"),
+    ("lw_attn8.hip", "hip"),
+    ("lw_pages.hip", "hip"),
     ("lw_runtime.cpp", "hiphost"),
     ("lw_attn_api.cpp", "hiphost"),
     ("lw_codec.cpp", "cxx"),

@@ -1,5 +1,6 @@
 // Attention over a paged key-value cache: arguments of the kernels and their launchers (host interface of
-// lw_attn_decode.hip and lw_attn_prompt.hip; the C-ABI in lw_attn_api.cpp checks what a caller gives and fills these).
+// lw_attn_decode.hip and lw_attn_prompt.hip, of lw_attn8.hip over a cache in 8 bits and of lw_pages.hip; the C-ABI in
+// lw_attn_api.cpp checks what a caller gives and fills these).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -85,8 +86,38 @@ int64_t prompt_items(int seqs, int kv_heads, int group, int tokens);
 size_t prompt_slot_bytes(int head_dim);
 int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots);
 
+// A cache in 8 bits: KvView's k and v are of bytes, its strides in bytes, and each 16 rows of a head have an exponent at
+// k (v) + page * pstride + head * hstride + row / 16.
+struct KvExps {
+  int8_t *k, *v;
+  int64_t pstride, hstride;
+};
+constexpr int kExpBlock = 16, kMostExp = 48;  // rows that share an exponent; exponents are -kMostExp .. kMostExp
+
+struct Append8Args {
+  AppendArgs a;
+  KvExps e;
+};
+struct Attn8Args {
+  AttnArgs a;
+  KvExps e;
+};
+
+// A step of sequences over their pages (lw_pages_advance)
+constexpr int kMostPageSeqs = 8192;
+struct PagesArgs {
+  int32_t *table, *free;
+  const int32_t *kv_len, *left, *add, *keep;
+  int32_t *kv_len_out, *left_out, *q_start, *position, *count;
+  int64_t *slot, tstride;
+  int seqs, table_pages, pages, page_shift, rows;
+};
+
 hipError_t launch_append(const AppendArgs& a, int head_dim, int type, int x_type, hipStream_t s);
 hipError_t launch_attn_decode(const AttnArgs& a, const DecodePlan& p, int head_dim, int type, hipStream_t s);
 hipError_t launch_attn_prompt(const AttnArgs& a, int head_dim, int type, hipStream_t s);
+hipError_t launch_append8(const Append8Args& a, int head_dim, int q_type, int x_type, hipStream_t s);
+hipError_t launch_attn8(const Attn8Args& a, int head_dim, int q_type, hipStream_t s);
+hipError_t launch_pages(const PagesArgs& a, hipStream_t s);
 
 }  // namespace lw

@@ -46,6 +46,26 @@ std::string check(const lw_kv_cache* c, const lw_batch* b, int heads) {
   return "";
 }
 
+// an 8-bit cache's shape as that of a cache of 16 bits (strides in elements), for what both have to keep to
+lw_kv_cache shape(const lw_kv8_cache& c) {
+  return {c.k, c.v, c.pages, c.page_stride, c.head_stride, c.row_stride, c.page_size, c.kv_heads, c.head_dim, LW_F16};
+}
+
+std::string check8(const lw_kv8_cache* c, const lw_batch* b, int heads) {
+  if (!c) return "no cache or no batch";
+  const lw_kv_cache plain = shape(*c);
+  const std::string bad = check(&plain, b, heads);
+  if (!bad.empty()) return bad;
+  if (c->page_size < lw::kExpBlock) return "pages of an 8-bit cache have 16 rows at least";
+  if (c->page_stride % 16 || c->head_stride % 16 || c->row_stride % 16) return "strides of an 8-bit cache must be multiples of 16 bytes";
+  if (c->pages > 0 && (!c->k_exp || !c->v_exp)) return "no exponents";
+  if (c->exp_page_stride < 0 || c->exp_head_stride < 0) return "negative stride of exponents";
+  if (c->reserved) return "reserved must be 0";
+  return "";
+}
+
+lw::KvExps exponents(const lw_kv8_cache& c) { return {c.k_exp, c.v_exp, c.exp_page_stride, c.exp_head_stride}; }
+
 lw::KvView view(const lw_kv_cache& c, const lw_batch& b) {
   lw::KvView v;
   v.k = static_cast<uint16_t*>(c.k);
@@ -108,6 +128,58 @@ int attention_args(const char* fn, const lw_kv_cache* cache, const lw_batch* bat
   return 0;
 }
 
+// what lw_kv_append and lw_kv8_append check alike; 1: nothing to do
+int append_args(const char* fn, const lw_kv_cache* cache, const lw_batch* batch, int heads, const void* q, const void* k,
+                const void* v, int x_type, long long ldq, long long ldk, long long ldv, const float* cos, const float* sin, int rot,
+                int rope_rows, int neighbours, void* q_out, long long ldo, lw::AppendArgs& a) {
+  if (x_type != LW_F32 && x_type != LW_F16 && x_type != LW_BF16) return refuse(fn, "unknown type of q, k and v");
+  if (neighbours != 0 && neighbours != 1) return refuse(fn, "neighbours must be 0 or 1");
+  if (rot < 0 || rot > cache->head_dim || rot % 8) return refuse(fn, "rot must be a multiple of 8 up to head_dim");
+  if (rot > 0 && (!cos || !sin || !aligned(cos, 0) || !aligned(sin, 0)))
+    return refuse(fn, "cos and sin must be given, aligned to 16 bytes");
+  if (rot > 0 && rope_rows < batch->max_kv) return refuse(fn, "cos and sin have fewer rows than max_kv");
+  if (batch->seqs == 0 || batch->tokens == 0) return 1;
+  const long long kd = (long long)cache->kv_heads * cache->head_dim, qd = (long long)heads * cache->head_dim;
+  if (!k || !v || (q && !q_out)) return refuse(fn, "null buffer");
+  if (!aligned(k, ldk) || !aligned(v, ldv) || ldk < kd || ldv < kd ||
+      (q && (!aligned(q, ldq) || !aligned(q_out, ldo) || ldq < qd || ldo < qd)))
+    return refuse(fn, "q, k, v and q_out must be aligned to 16 bytes, with row strides of multiples of 8 that hold their heads");
+  const long long parts = (qd + 2 * kd + 8 * 256 - 1) / (8 * 256);
+  if (parts * batch->tokens > kMostBlocks) return refuse(fn, "more tokens than a launch can take");
+  a.c = view(*cache, *batch);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.ldq = ldq;
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.ldo = ldo;
+  a.q_out = static_cast<uint16_t*>(q_out);
+  a.cos = cos;
+  a.sin = sin;
+  a.heads = heads;
+  a.rot = rot;
+  a.rope_rows = rope_rows > 0 ? rope_rows : 1;
+  a.neighbours = neighbours;
+  return 0;
+}
+
+// lw_attn8_decode and lw_attn8_prompt
+int attend8(const char* fn, bool decode, const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, int q_type,
+            long long ldq, void* out, int out_type, long long ldo, float scale, int window, void* stream) {
+  const std::string bad = check8(cache, batch, heads);
+  if (!bad.empty()) return refuse(fn, bad);
+  if (q_type != LW_F16 && q_type != LW_BF16) return refuse(fn, "the type of q must be LW_F16 or LW_BF16");
+  lw::Attn8Args a;
+  const lw_kv_cache plain = shape(*cache);
+  const int rc = attention_args(fn, &plain, batch, heads, q, ldq, out, out_type, ldo, scale, window, a.a);
+  if (rc) return rc < 0 ? -1 : 0;
+  a.e = exponents(*cache);
+  if (decode && batch->max_new < 1) return 0;
+  if (decode && batch->max_new > 16) return refuse(fn, "max_new is more than 16 (lw_attn8_prompt takes any number)");
+  return launched(fn, lw::launch_attn8(a, cache->head_dim, q_type, static_cast<hipStream_t>(stream)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -129,36 +201,9 @@ int lw_kv_append(const lw_kv_cache* cache, const lw_batch* batch, int heads, con
   const char* fn = "lw_kv_append";
   const std::string bad = check(cache, batch, heads);
   if (!bad.empty()) return refuse(fn, bad);
-  if (x_type != LW_F32 && x_type != LW_F16 && x_type != LW_BF16) return refuse(fn, "unknown type of q, k and v");
-  if (neighbours != 0 && neighbours != 1) return refuse(fn, "neighbours must be 0 or 1");
-  if (rot < 0 || rot > cache->head_dim || rot % 8) return refuse(fn, "rot must be a multiple of 8 up to head_dim");
-  if (rot > 0 && (!cos || !sin || !aligned(cos, 0) || !aligned(sin, 0)))
-    return refuse(fn, "cos and sin must be given, aligned to 16 bytes");
-  if (rot > 0 && rope_rows < batch->max_kv) return refuse(fn, "cos and sin have fewer rows than max_kv");
-  if (batch->seqs == 0 || batch->tokens == 0) return 0;
-  const long long kd = (long long)cache->kv_heads * cache->head_dim, qd = (long long)heads * cache->head_dim;
-  if (!k || !v || (q && !q_out)) return refuse(fn, "null buffer");
-  if (!aligned(k, ldk) || !aligned(v, ldv) || ldk < kd || ldv < kd ||
-      (q && (!aligned(q, ldq) || !aligned(q_out, ldo) || ldq < qd || ldo < qd)))
-    return refuse(fn, "q, k, v and q_out must be aligned to 16 bytes, with row strides of multiples of 8 that hold their heads");
-  const long long parts = (qd + 2 * kd + 8 * 256 - 1) / (8 * 256);
-  if (parts * batch->tokens > kMostBlocks) return refuse(fn, "more tokens than a launch can take");
   lw::AppendArgs a;
-  a.c = view(*cache, *batch);
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.ldq = ldq;
-  a.ldk = ldk;
-  a.ldv = ldv;
-  a.ldo = ldo;
-  a.q_out = static_cast<uint16_t*>(q_out);
-  a.cos = cos;
-  a.sin = sin;
-  a.heads = heads;
-  a.rot = rot;
-  a.rope_rows = rope_rows > 0 ? rope_rows : 1;
-  a.neighbours = neighbours;
+  const int rc = append_args(fn, cache, batch, heads, q, k, v, x_type, ldq, ldk, ldv, cos, sin, rot, rope_rows, neighbours, q_out, ldo, a);
+  if (rc) return rc < 0 ? -1 : 0;
   return launched(fn, lw::launch_append(a, cache->head_dim, cache->type, x_type, static_cast<hipStream_t>(stream)));
 }
 
@@ -208,6 +253,74 @@ int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
   const int most_kv = a.window > 0 ? std::min(batch->max_kv, a.window) : batch->max_kv;
   a.most_run = most_kv / a.splits;
   return launched(fn, lw::launch_attn_prompt(a, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
+}
+
+long long lw_attn8_workspace(const lw_kv8_cache* cache, const lw_batch* batch, int heads) {
+  const std::string bad = check8(cache, batch, heads);
+  if (!bad.empty()) return refuse("lw_attn8_workspace", bad);
+  const lw_kv_cache plain = shape(*cache);
+  return lw_attn_workspace(&plain, batch, heads);
+}
+
+int lw_kv8_append(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, const void* k, const void* v,
+                  int x_type, long long ldq, long long ldk, long long ldv, const float* cos, const float* sin, int rot,
+                  int rope_rows, int neighbours, void* q_out, int q_type, long long ldo, void* stream) {
+  const char* fn = "lw_kv8_append";
+  const std::string bad = check8(cache, batch, heads);
+  if (!bad.empty()) return refuse(fn, bad);
+  if (q_type != LW_F16 && q_type != LW_BF16) return refuse(fn, "the type of q_out must be LW_F16 or LW_BF16");
+  lw::Append8Args a;
+  const lw_kv_cache plain = shape(*cache);
+  const int rc = append_args(fn, &plain, batch, heads, q, k, v, x_type, ldq, ldk, ldv, cos, sin, rot, rope_rows, neighbours, q_out, ldo, a.a);
+  if (rc) return rc < 0 ? -1 : 0;
+  if (((long long)batch->tokens / lw::kExpBlock + 2ll * batch->seqs) * 2 * cache->kv_heads + (long long)batch->tokens * ((heads + 15) / 16) > kMostBlocks)
+    return refuse(fn, "more tokens than a launch can take");
+  a.e = exponents(*cache);
+  return launched(fn, lw::launch_append8(a, cache->head_dim, q_type, x_type, static_cast<hipStream_t>(stream)));
+}
+
+int lw_attn8_decode(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, int q_type, long long ldq,
+                    void* out, int out_type, long long ldo, float scale, int window, void* stream) {
+  return attend8("lw_attn8_decode", true, cache, batch, heads, q, q_type, ldq, out, out_type, ldo, scale, window, stream);
+}
+
+int lw_attn8_prompt(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, int q_type, long long ldq,
+                    void* out, int out_type, long long ldo, float scale, int window, void* stream) {
+  return attend8("lw_attn8_prompt", false, cache, batch, heads, q, q_type, ldq, out, out_type, ldo, scale, window, stream);
+}
+
+int lw_pages_advance(const lw_pages* p, const int32_t* new_tokens, const int32_t* keep, int rows, int32_t* kv_len_out,
+                     int32_t* left_out, int32_t* q_start, int32_t* position, int64_t* slot, void* stream) {
+  const char* fn = "lw_pages_advance";
+  if (!p) return refuse(fn, "no pages");
+  if (p->seqs < 0 || p->seqs > lw::kMostPageSeqs) return refuse(fn, "up to 8192 sequences");
+  if (p->page_size < 1 || p->page_size > 65536 || (p->page_size & (p->page_size - 1)))
+    return refuse(fn, "page_size must be a power of two up to 65536");
+  if (p->pages < 0 || p->pages >= kMostRows || rows < 0 || rows >= kMostRows) return refuse(fn, "pages or rows out of range");
+  if (p->table_pages < 0 || p->table_stride < p->table_pages || (long long)p->table_pages * p->page_size >= kMostRows)
+    return refuse(fn, "the table holds 2^30 positions or more, or its stride is less than its pages");
+  if (!q_start || !left_out || !p->left || !p->workspace || (p->pages > 0 && !p->free)) return refuse(fn, "null array");
+  if (p->seqs > 0 && (!p->kv_len || !kv_len_out || !new_tokens || (p->table_pages > 0 && !p->table))) return refuse(fn, "null array");
+  lw::PagesArgs a;
+  a.table = p->table;
+  a.free = p->free;
+  a.kv_len = p->kv_len;
+  a.left = p->left;
+  a.add = new_tokens;
+  a.keep = keep;
+  a.kv_len_out = kv_len_out;
+  a.left_out = left_out;
+  a.q_start = q_start;
+  a.position = position;
+  a.count = p->workspace;
+  a.slot = slot;
+  a.tstride = p->table_stride;
+  a.seqs = p->seqs;
+  a.table_pages = p->table_pages;
+  a.pages = p->pages;
+  a.page_shift = __builtin_ctz((unsigned)p->page_size);
+  a.rows = rows;
+  return launched(fn, lw::launch_pages(a, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

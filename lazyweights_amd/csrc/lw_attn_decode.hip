@@ -16,14 +16,6 @@ namespace {
 // Bound by memory: 16383 tokens of 32 + 8 + 8 heads of 128, fp32 in, 612 MB in 109 us (5.6 TB/s, two thirds of it read; a copy of
 // 1 GiB reaches 5.0). A few tokens are one pass of loads that depend on each other (the sequence, its length, the page):
 // 2.5 us for one token, 3.4 for 48 sequences, less than the 8 us that the host takes to make the call.
-template <int X, bool BF>  // X: type of q, k, v (LW_F32, LW_F16, LW_BF16)
-__device__ __forceinline__ f4v load4(const void* p, int64_t i) {
-  if (X == 0) return *reinterpret_cast<const f4v*>(static_cast<const float*>(p) + i);
-  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-  return (f4v){wide<X == 2>((uint16_t)u.x), wide<X == 2>((uint16_t)(u.x >> 16)), wide<X == 2>((uint16_t)u.y),
-               wide<X == 2>((uint16_t)(u.y >> 16))};
-}
-
 template <int D, int X, bool BF>
 __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
   constexpr int U = D / 8;
@@ -43,7 +35,7 @@ __global__ __launch_bounds__(256) void k_kv_append(const AppendArgs a) {
   const int64_t at = (what == 0 ? a.ldq : what == 1 ? a.ldk : a.ldv) * row + (int64_t)h * D;
   const bool turn = what < 2 && 8 * u < a.rot;
   const int e0 = turn && !a.neighbours ? 4 * u : 8 * u, e1 = turn && !a.neighbours ? a.rot / 2 + 4 * u : 8 * u + 4;
-  f4v x = load4<X, BF>(src, at + e0), y = load4<X, BF>(src, at + e1);
+  f4v x = load4<X>(src, at + e0), y = load4<X>(src, at + e1);
   if (turn) {
     const int64_t r = (int64_t)min(pos, a.rope_rows - 1) * (a.rot / 2) + 4 * u;
     const f4v c = *reinterpret_cast<const f4v*>(a.cos + r), n = *reinterpret_cast<const f4v*>(a.sin + r);

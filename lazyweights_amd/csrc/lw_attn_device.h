@@ -132,6 +132,15 @@ __device__ __forceinline__ int64_t key_offset(const KvView& c, uint32_t page, in
   return (there ? (int64_t)page * c.pstride : 0) + (int64_t)(key & ((1 << c.page_shift) - 1)) * c.rstride;
 }
 
+// 4 elements of type X (LW_F32, LW_F16, LW_BF16) from i on
+template <int X>
+__device__ __forceinline__ f4v load4(const void* p, int64_t i) {
+  if (X == 0) return *reinterpret_cast<const f4v*>(static_cast<const float*>(p) + i);
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+  return (f4v){wide<X == 2>((uint16_t)u.x), wide<X == 2>((uint16_t)(u.x >> 16)), wide<X == 2>((uint16_t)u.y),
+               wide<X == 2>((uint16_t)(u.y >> 16))};
+}
+
 template <int OUT>
 __device__ __forceinline__ void store4(void* out, int64_t i, f4v v) {
   if (OUT == 0)
