@@ -283,7 +283,8 @@ int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
  * r * row_stride of k (v) and holds head_dim (64, 96 or 128) numbers of 1 sign, 4 exponent and 3 mantissa bits (OCP e4m3: up to 448,
  * no infinities); each block of 16 rows of a head has an exponent e in k_exp (v_exp)[p * exp_page_stride + h *
  * exp_head_stride + r / 16], -48 to 48 (others are taken as the nearer of these): an element is its number times 2^e.
- * Pages of page_size rows, a power of two from 16 to 65536; byte strides are multiples of 16, k and v aligned to 16 bytes. Calls
+ * Pages of page_size rows, a power of two from 16 to 65536; byte strides are multiples of 16 (row_stride less than 2^26), k and
+ * v aligned to 16 bytes. Calls
  * are made with the cache's GPU as the calling thread's current one, where `stream` is. */
 typedef struct lw_kv8_cache {
   void* k;

@@ -35,6 +35,7 @@ SOURCES = [
     ("lw_attn_decode.hip", "hip"),
     ("lw_attn_prompt.hip", "hip"),
     ("lw_attn8.hip", "hip"),
+    ("lw_attn8_decode.hip", "hip"),
     ("lw_pages.hip", "hip"),
     ("lw_runtime.cpp", "hiphost"),
     ("lw_attn_api.cpp", "hiphost"),

@@ -77,6 +77,7 @@ struct DecodePlan {
   size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
 };
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);
+DecodePlan decode8_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);  // of an 8-bit cache
 
 // The prompt kernel's row tiles of 128 (token, head) rows of a key-value head, and into how many blocks the keys of each are shared
 // out, with a workspace of `slots` slots of prompt_slot_bytes() each (kPromptSlots are of use).
@@ -117,6 +118,7 @@ hipError_t launch_append(const AppendArgs& a, int head_dim, int type, int x_type
 hipError_t launch_attn_decode(const AttnArgs& a, const DecodePlan& p, int head_dim, int type, hipStream_t s);
 hipError_t launch_attn_prompt(const AttnArgs& a, int head_dim, int type, hipStream_t s);
 hipError_t launch_append8(const Append8Args& a, int head_dim, int q_type, int x_type, hipStream_t s);
+hipError_t launch_attn8_decode(const Attn8Args& a, const DecodePlan& p, int head_dim, int q_type, hipStream_t s);
 hipError_t launch_attn8(const Attn8Args& a, int head_dim, int q_type, hipStream_t s);
 hipError_t launch_pages(const PagesArgs& a, hipStream_t s);
 

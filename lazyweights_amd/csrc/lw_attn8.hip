@@ -1,15 +1,12 @@
 // Appending to a paged key-value cache held in 8 bits, and attention over it.
 #include <algorithm>
 
-#include "lw_attn_device.h"
+#include "lw_attn8_device.h"
 
 namespace lw {
 
 namespace {
 
-typedef int i32x2 __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 __device__ __forceinline__ int exponent(int8_t e) { return clampi(e, -kMostExp, kMostExp); }
 
 // The least e with most <= 448 2^e, 448 = 1.75 * 2^8: of a magnitude 1.f 2^k that is k - 8, and one more past 1.75
@@ -23,10 +20,6 @@ __device__ __forceinline__ uint32_t to8(f4v v) {
   for (int i = 0; i < 4; ++i) v[i] = finite(v[i]) ? fminf(fmaxf(v[i], -448.f), 448.f) : NAN;
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], w, true);
-}
-__device__ __forceinline__ f4v from8(uint32_t w) {
-  const f2v a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  return (f4v){a[0], a[1], b[0], b[1]};
 }
 
 // x and y, pairs (x, y) or, as neighbours, pairs within each, by the angles c, n: every product and sum rounded for itself

@@ -59,6 +59,7 @@ std::string check8(const lw_kv8_cache* c, const lw_batch* b, int heads) {
   if (c->page_size < lw::kExpBlock) return "pages of an 8-bit cache have 16 rows at least";
   if (c->page_stride % 16 || c->head_stride % 16 || c->row_stride % 16) return "strides of an 8-bit cache must be multiples of 16 bytes";
   if (c->pages > 0 && (!c->k_exp || !c->v_exp)) return "no exponents";
+  if (c->row_stride >= 1 << 26) return "rows of an 8-bit cache lie less than 2^26 bytes apart";
   if (c->exp_page_stride < 0 || c->exp_head_stride < 0) return "negative stride of exponents";
   if (c->reserved) return "reserved must be 0";
   return "";
@@ -164,6 +165,21 @@ int append_args(const char* fn, const lw_kv_cache* cache, const lw_batch* batch,
   return 0;
 }
 
+// the plan and the batch's workspace into the decode kernel's arguments
+bool take_plan(const char* fn, const lw::DecodePlan& p, const lw_batch* batch, lw::AttnArgs& a) {
+  if (p.most_keys < batch->max_kv) return refuse(fn, "more sequences, heads and positions than a launch can take"), false;
+  if (!batch->workspace || (reinterpret_cast<uintptr_t>(batch->workspace) & 15) ||
+      batch->workspace_bytes < (long long)(p.count_bytes + p.part_bytes))
+    return refuse(fn, "needs a workspace of " + std::to_string(p.count_bytes + p.part_bytes) + " bytes, aligned to 16"), false;
+  a.count = static_cast<uint32_t*>(batch->workspace);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(batch->workspace) + p.count_bytes);
+  a.row_blocks = p.row_blocks;
+  a.blocks_log2 = p.blocks_log2;
+  a.whole = p.whole;
+  a.most_keys = p.most_keys;
+  return true;
+}
+
 // lw_attn8_decode and lw_attn8_prompt
 int attend8(const char* fn, bool decode, const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, int q_type,
             long long ldq, void* out, int out_type, long long ldo, float scale, int window, void* stream) {
@@ -177,6 +193,11 @@ int attend8(const char* fn, bool decode, const lw_kv8_cache* cache, const lw_bat
   a.e = exponents(*cache);
   if (decode && batch->max_new < 1) return 0;
   if (decode && batch->max_new > 16) return refuse(fn, "max_new is more than 16 (lw_attn8_prompt takes any number)");
+  if (decode) {
+    const lw::DecodePlan p = lw::decode8_plan(batch->seqs, cache->kv_heads, a.a.group, cache->head_dim, batch->max_new, batch->max_kv);
+    if (!take_plan(fn, p, batch, a.a)) return -1;
+    return launched(fn, lw::launch_attn8_decode(a, p, cache->head_dim, q_type, static_cast<hipStream_t>(stream)));
+  }
   return launched(fn, lw::launch_attn8(a, cache->head_dim, q_type, static_cast<hipStream_t>(stream)));
 }
 
@@ -217,16 +238,7 @@ int lw_attn_decode(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
   if (batch->max_new > 16) return refuse(fn, "max_new is more than 16 (lw_attn_prompt takes any number)");
   const lw::DecodePlan p = lw::decode_plan(batch->seqs, cache->kv_heads, a.group, cache->head_dim, batch->max_new,
                                            batch->max_kv);
-  if (p.most_keys < batch->max_kv) return refuse(fn, "more sequences, heads and positions than a launch can take");
-  if (!batch->workspace || (reinterpret_cast<uintptr_t>(batch->workspace) & 15) ||
-      batch->workspace_bytes < (long long)(p.count_bytes + p.part_bytes))
-    return refuse(fn, "needs a workspace of " + std::to_string(p.count_bytes + p.part_bytes) + " bytes, aligned to 16");
-  a.count = static_cast<uint32_t*>(batch->workspace);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(batch->workspace) + p.count_bytes);
-  a.row_blocks = p.row_blocks;
-  a.blocks_log2 = p.blocks_log2;
-  a.whole = p.whole;
-  a.most_keys = p.most_keys;
+  if (!take_plan(fn, p, batch, a)) return -1;
   return launched(fn, lw::launch_attn_decode(a, p, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
 }
 
@@ -258,8 +270,11 @@ int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
 long long lw_attn8_workspace(const lw_kv8_cache* cache, const lw_batch* batch, int heads) {
   const std::string bad = check8(cache, batch, heads);
   if (!bad.empty()) return refuse("lw_attn8_workspace", bad);
-  const lw_kv_cache plain = shape(*cache);
-  return lw_attn_workspace(&plain, batch, heads);
+  if (batch->seqs == 0) return 0;
+  if (batch->max_new > 16) return 0;
+  const lw::DecodePlan p = lw::decode8_plan(batch->seqs, cache->kv_heads, heads / cache->kv_heads, cache->head_dim, batch->max_new,
+                                            batch->max_kv);
+  return (long long)(p.count_bytes + p.part_bytes);
 }
 
 int lw_kv8_append(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, const void* k, const void* v,
