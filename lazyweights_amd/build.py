@@ -34,8 +34,9 @@ SOURCES = [
     ("lw_prefill.hip", "hip"),
     ("lw_attn_decode.hip", "hip"),
     ("lw_attn_prompt.hip", "hip"),
-    ("lw_attn8.hip", "hip"),
+    ("lw_kv8_append.hip", "hip"),
     ("lw_attn8_decode.hip", "hip"),
+    ("lw_attn8_prompt.hip", "hip"),
     ("lw_pages.hip", "hip"),
     ("lw_runtime.cpp", "hiphost"),
     ("lw_attn_api.cpp", "hiphost"),

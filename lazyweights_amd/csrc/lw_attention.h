@@ -39,13 +39,13 @@ struct AppendArgs {
 // above d, is less than 2^31 too large
 struct Divisor {
   uint64_t mul;
-  int shift;
+  int shift, of;
   __host__ __device__ int operator()(int x) const { return (int)(((uint64_t)(uint32_t)x * mul) >> shift); }
 };
 inline Divisor divisor(int d) {
   int k = 0;
   while ((1u << k) < (uint32_t)d) ++k;
-  return {(((uint64_t)1 << (31 + k)) + d - 1) / d, 31 + k};
+  return {(((uint64_t)1 << (31 + k)) + d - 1) / d, 31 + k, d};
 }
 
 struct AttnArgs {
@@ -73,7 +73,8 @@ struct AttnArgs {
 // most_keys is the most of a sequence that keeps it there (2^31 tiles in all).
 struct DecodePlan {
   int row_tiles, row_blocks, blocks, blocks_log2, most_keys;
-  bool whole;  // a block per item, of 8 waves
+  bool whole;  // a block per item (of 16 bits: of 8 waves)
+  int spare;   // (8 bits) blocks beyond one for every item
   size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
 };
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);
@@ -102,6 +103,7 @@ struct Append8Args {
 struct Attn8Args {
   AttnArgs a;
   KvExps e;
+  Divisor by_spare;  // decode: the launch's blocks beyond one for every item
 };
 
 // A step of sequences over their pages (lw_pages_advance)
@@ -119,7 +121,7 @@ hipError_t launch_attn_decode(const AttnArgs& a, const DecodePlan& p, int head_d
 hipError_t launch_attn_prompt(const AttnArgs& a, int head_dim, int type, hipStream_t s);
 hipError_t launch_append8(const Append8Args& a, int head_dim, int q_type, int x_type, hipStream_t s);
 hipError_t launch_attn8_decode(const Attn8Args& a, const DecodePlan& p, int head_dim, int q_type, hipStream_t s);
-hipError_t launch_attn8(const Attn8Args& a, int head_dim, int q_type, hipStream_t s);
+hipError_t launch_attn8_prompt(const Attn8Args& a, int head_dim, int q_type, hipStream_t s);
 hipError_t launch_pages(const PagesArgs& a, hipStream_t s);
 
 }  // namespace lw

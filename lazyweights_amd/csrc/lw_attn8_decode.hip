@@ -8,15 +8,143 @@ namespace lw {
 
 namespace {
 
-// Tiles [t_from, t_to) of 16 H keys of the item (s, kvh, rb), as decode_item's of a 16-bit cache.
-template <int D, bool BF, int RT, int NW, int H>
-__device__ __forceinline__ void decode8_item(const Attn8Args& args, uint8_t* smem, float* ml, float* pcare, int* last_block, int s,
-                                             const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0, int T,
-                                             uint32_t run, int lane, int w, int n, int g) {
-  constexpr int KEYS = 16 * H, C = D / 32, DT = D / 16, NP = 2, FULL = D / 64, TAIL = C % 2;
-  constexpr float LIFT = lift<false>(0);
+// The part of an item that a block has. Items are (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as
+// many tiles of KEYS keys as the sequence's rows see together. Of a list of all items' tiles a part takes `run` at most, total /
+// spare, so that items + spare blocks are enough whatever the lengths; parts of one item alone, so that a block has one pass, one
+// join and is done, and what it waits for in turn is covered by the blocks beside it. (Equal runs of the list for a block
+// per place on the card, as for 16 bits, have a block go from item to item, each waited for anew: us with runs / parts, 256 sequences of
+// 100-2000 keys, 8 heads of 128: 119 / 91, 30 of them 29 / 19, one of 30000 26 / 20.)
+struct Part {
+  Seq sq;
+  int s, kvh, rb, lo, t_from, t_to;
+  int base_slot, part, active;
+};
+template <int NW, int KEYS>
+__device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles_l, uint32_t* parts_l, int lane, int w, Part& p) {
   const AttnArgs& a = args.a;
   const KvView& c = a.c;
+  const int seqs = c.seqs, kv_heads = c.kv_heads, H = kv_heads * a.row_blocks, chunks = (seqs + 63) >> 6;
+  // tiles of each of a sequence's items: those of the keys [lo, len) that its rows see; one where they see none, to write
+  // the zeros
+  auto first_key = [&](const Seq& q) { return a.window > 0 ? max(0, q.len - q.rows - a.window + 1) & ~(KEYS - 1) : 0; };
+  auto tiles_of = [&](const Seq& q) { return q.rows ? max((q.len - first_key(q) + KEYS - 1) / KEYS, 1) : 0; };
+  p.base_slot = p.part = 0;
+  p.active = 1;
+  if (a.whole) {
+    p.s = (int)blockIdx.x / H;
+    const int hb = (int)blockIdx.x - p.s * H;
+    p.rb = hb / kv_heads;
+    p.kvh = hb - p.rb * kv_heads;
+    p.sq = sequence(c, p.s);
+    p.lo = first_key(p.sq);
+    p.t_from = 0;
+    p.t_to = tiles_of(p.sq);
+    return p.t_to > 0;
+  }
+  // the sequences are held 64 at a time, one per lane, with their tiles and parts and those up to theirs
+  Seq mine = {0, 0, 0};
+  uint32_t T = 0, tiles = 0, parts = 0;
+  auto hold = [&](int chunk) __attribute__((always_inline)) {
+    mine = {0, 0, 0};
+    if (64 * chunk + lane < seqs) {
+      mine = sequence(c, 64 * chunk + lane);
+      mine.len = min(mine.len, a.most_keys);
+    }
+    T = tiles_of(mine);
+  };
+  auto upto = [&](uint32_t v) __attribute__((always_inline)) {
+    for (int d = 1; d < min(64, seqs); d *= 2) {
+      const uint32_t o = __shfl_up(v, d);
+      if (lane >= d) v += o;
+    }
+    return v;
+  };
+  auto run_of = [&](uint32_t total) { return max((uint32_t)args.by_spare((int)total + args.by_spare.of - 1), (uint32_t)NW); };
+  uint32_t run, tiles_before = 0, parts_before = 0, at = blockIdx.x;
+  int chunk = 0;
+  if (chunks == 1) {
+    hold(0);
+    tiles = upto(T * H);
+    run = run_of(__builtin_amdgcn_readlane(tiles, min(seqs, 64) - 1));
+    parts = upto((T + run - 1) / run * H);
+  } else {
+    // sums up to each 64th sequence, of tiles and then, with the run that these give, of parts
+    auto sums = [&](uint32_t* l, auto value) __attribute__((always_inline)) {
+      for (int i = w; i < chunks; i += NW) {
+        hold(i);
+        const uint32_t v = upto(value());
+        if (lane == 63) l[i] = v;
+      }
+      __syncthreads();
+      if (w == 0) {
+        uint32_t base = 0;
+        for (int i = 0; i < chunks; i += 64) {
+          uint32_t t = i + lane < chunks ? l[i + lane] : 0;
+#pragma unroll
+          for (int d = 1; d < 64; d *= 2) {
+            const uint32_t o = __shfl_up(t, d);
+            if (lane >= d) t += o;
+          }
+          t += base;
+          if (i + lane < chunks) l[i + lane] = t;
+          base = __builtin_amdgcn_readlane(t, 63);
+        }
+      }
+      __syncthreads();
+    };
+    sums(tiles_l, [&] { return T * H; });
+    run = run_of(__builtin_amdgcn_readfirstlane(tiles_l[chunks - 1]));
+    sums(parts_l, [&] { return (T + run - 1) / run * H; });
+    for (int i = 0; i < chunks; i += 64) chunk += __popcll(__ballot(i + lane < chunks && parts_l[min(i + lane, chunks - 1)] <= at));
+    if (chunk && chunk < chunks) {
+      tiles_before = __builtin_amdgcn_readfirstlane(tiles_l[chunk - 1]);
+      parts_before = __builtin_amdgcn_readfirstlane(parts_l[chunk - 1]);
+    }
+    __syncthreads();  // (the memory is used again)
+    if (chunk >= chunks) return false;
+    hold(chunk);
+    tiles = upto(T * H);
+    parts = upto((T + run - 1) / run * H);
+  }
+  at -= parts_before;
+  const int j = __ffsll((unsigned long long)__ballot(parts > at)) - 1;
+  if (j < 0) return false;
+  auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane(v, j); };
+  p.sq = Seq{(int)of(mine.row0), (int)of(mine.rows), (int)of(mine.len)};
+  p.s = 64 * chunk + j;
+  const uint32_t t = of(T), each = (t + run - 1) / run;
+  at -= of(parts) - each * H;
+  tiles_before += of(tiles) - t * H;
+  const uint32_t hb = at / each;
+  p.rb = hb / kv_heads;
+  p.kvh = hb - p.rb * kv_heads;
+  p.part = at - hb * each;
+  p.active = each;
+  p.base_slot = (tiles_before + hb * t) / run;  // (two items' first parts, of runs at least, have not one number)
+  p.lo = first_key(p.sq);
+  p.t_from = p.part * run;
+  p.t_to = min(p.t_from + run, t);
+  return true;
+}
+
+template <int D, bool BF, int RT, int NW, int H>
+__global__ __launch_bounds__(64 * NW, RT == 1 ? 4 : 2) void k_attn8_decode(const Attn8Args args) {
+  constexpr int KEYS = 16 * H, C = D / 32, DT = D / 16, NP = 2, FULL = D / 64, TAIL = C % 2;
+  constexpr float LIFT = lift<false>(0);
+  // the waves' V tiles, and behind each the weights of 32 keys of the careful pass (after the loop their sums); then, of more than one
+  // row tile, q
+  constexpr int WAVE = std::max(KEYS * D + 32 * 16 * 4, 64 * D);
+  __shared__ __align__(16) uint8_t smem[NW * WAVE + (RT > 1 ? NW * RT * 16 * D * 2 : 0)];
+  __shared__ float ml[NW * 16 * RT * 2];
+  __shared__ int last_block;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  const AttnArgs& a = args.a;
+  const KvView& c = a.c;
+  Part p0;
+  uint32_t* sums_l = reinterpret_cast<uint32_t*>(smem);  // of tiles and of parts of the sequences up to each 64th
+  if (!find_part<NW, KEYS>(args, sums_l, sums_l + 1024, lane, w, p0)) return;
+  const Seq& sq = p0.sq;
+  const int s = p0.s, kvh = p0.kvh, rb = p0.rb, lo = p0.lo, t_from = p0.t_from, t_to = p0.t_to;
   const Divisor by_group = a.by_group;
   const int R = sq.rows * a.group, r0 = rb * RT * 16;
   const int past = sq.len - sq.rows;  // row r has position past + r / group
@@ -30,7 +158,7 @@ __device__ __forceinline__ void decode8_item(const Attn8Args& args, uint8_t* sme
   // 64 i + 16 g on, operands 2 i and 2 i + 1 (a tail of 32 dims: 8 bytes), and q's are of the same dims.
   constexpr bool QL = RT > 1;
   u32x4 qr[QL ? 1 : C];
-  u32x4* ql = reinterpret_cast<u32x4*>(smem + NW * KEYS * D + w * RT * 16 * D * 2) + lane;
+  u32x4* ql = reinterpret_cast<u32x4*>(smem + NW * WAVE + w * RT * 16 * D * 2) + lane;
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     // (past the last row: that row's q, for which nothing is written)
@@ -53,7 +181,7 @@ __device__ __forceinline__ void decode8_item(const Attn8Args& args, uint8_t* sme
   const int8_t* eb = (lane & 4 ? args.e.v : args.e.k) + kvh * args.e.hstride;
   // V of a tile, each wave's own: [H][D / 16 chunks][16 keys][16 dims], the keys of odd blocks turned by 8, so that the keys
   // 4 g .. 4 g + 3 of two blocks lie in other banks
-  uint8_t* vl = smem + w * KEYS * D;
+  uint8_t* vl = smem + w * WAVE;
 
   float m[RT], l[RT];  // m: the largest score plus its value's exponent, the power of two that weights are measured against
   f4v o[RT][DT];
@@ -176,7 +304,7 @@ __device__ __forceinline__ void decode8_item(const Attn8Args& args, uint8_t* sme
           for (int x = 0; x < H / 2; ++x) split8<false, NP>(p[r] + 8 * x, part[r][x]);
       }
       if constexpr (careful) {
-        float* pl = pcare + w * 32 * 16;  // [32 keys][16 rows]
+        float* pl = reinterpret_cast<float*>(vl + KEYS * D);  // [32 keys][16 rows]
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
@@ -222,30 +350,14 @@ __device__ __forceinline__ void decode8_item(const Attn8Args& args, uint8_t* sme
       for (int i = 0; i < 4; ++i) bad |= !finite(o[r][d][i]);
   if (__any(bad)) pass(std::true_type{});
 
-  join_item<D, RT, NW>(a, smem, ml, last_block, m, l, o, s, sq, kvh, rb, item0, T, run, w, n, g);
-}
-
-template <int D, bool BF, int RT, int NW, int H>
-__global__ __launch_bounds__(64 * NW, 2) void k_attn8_decode(const Attn8Args args) {
-  // V tiles of the waves (after the loop their sums), then, of more than one row tile, q
-  __shared__ __align__(16) uint8_t smem[NW * D * std::max(16 * H, 64) + (RT > 1 ? NW * RT * 16 * D * 2 : 0)];
-  __shared__ float ml[NW * 16 * RT * 2];
-  __shared__ float pcare[NW * 32 * 16];
-  __shared__ uint32_t csum[1024];  // tiles of the sequences up to each 64th
-  __shared__ int last_block;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  walk_items<NW, 16 * H>(args.a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0,
-                                                    int T, uint32_t run) __attribute__((always_inline)) {
-    decode8_item<D, BF, RT, NW, H>(args, smem, ml, pcare, &last_block, s, sq, kvh, rb, lo, t_from, t_to, item0, T, run, lane, w, n, g);
-  });
+  join_item<D, RT, NW>(a, smem, ml, &last_block, m, l, o, s, sq, kvh, rb, p0.base_slot, p0.part, p0.active, w, n, g);
 }
 
 template <int D, bool BF>
 hipError_t decode8_d(const Attn8Args& a, const DecodePlan& p, hipStream_t s) {
   const dim3 grid((uint32_t)p.blocks);
-  if (p.row_tiles == 1 && p.whole) k_attn8_decode<D, BF, 1, 8, 4><<<grid, 512, 0, s>>>(a);
-  else if (p.row_tiles == 1) k_attn8_decode<D, BF, 1, 4, 4><<<grid, 256, 0, s>>>(a);
-  else k_attn8_decode<D, BF, 2, 4, 4><<<grid, 256, 0, s>>>(a);
+  if (p.row_tiles == 1) k_attn8_decode<D, BF, 1, 4, 2><<<grid, 256, 0, s>>>(a);
+  else k_attn8_decode<D, BF, 2, 4, 2><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -256,19 +368,22 @@ DecodePlan decode8_plan(int seqs, int kv_heads, int group, int head_dim, int max
   const int rows = group * max_new;
   p.row_tiles = rows <= 16 || (int64_t)seqs * kv_heads * max_kv < 1 << 18 ? 1 : 2;
   p.row_blocks = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
-  const int64_t items = (int64_t)seqs * kv_heads * p.row_blocks, tiles = items * (max_kv / 64 + 2);
-  const int most = items > 256 ? 9 : 8;
-  p.whole = p.row_tiles == 1 && items <= 1 << 20 && (max_kv <= 512 || (items >= 1024 && max_kv <= 8192));
+  const int64_t items = (int64_t)seqs * kv_heads * p.row_blocks, tiles = items * (max_kv / 32 + 2);
+  const int64_t few = items <= 64 ? 256 - items : std::max<int64_t>(512 - items, 256);
+  const int64_t many = std::min<int64_t>(std::max<int64_t>(tiles / 96, 512), 2048);
+  p.whole = items <= 1 << 20 && (max_kv <= 256 || (items >= 1024 && max_kv <= 2048));
   p.blocks_log2 = 0;
-  while (p.blocks_log2 < most && ((int64_t)4 << p.blocks_log2) < tiles) ++p.blocks_log2;
-  p.blocks = p.whole ? (int)items : 1 << p.blocks_log2;
+  p.spare = (int)std::max<int64_t>(1, std::min<int64_t>(items > 256 ? many : few, (tiles + 3) / 4));
+  p.blocks = (int)items + (p.whole ? 0 : p.spare);
   p.count_bytes = ((size_t)items * 4 + 255) & ~(size_t)255;
-  p.part_bytes = ((size_t)1 << p.blocks_log2) * 2 * p.row_tiles * 16 * (head_dim + 2) * 4;
-  p.most_keys = (int)std::min<int64_t>(1 << 30, ((int64_t)1 << 37) / std::max<int64_t>(items, 1) / 2 - 128);
+  p.part_bytes = ((size_t)p.spare + 1) * 2 * p.row_tiles * 16 * (head_dim + 2) * 4;
+  p.most_keys = (int)std::min<int64_t>(1 << 30, ((int64_t)1 << 36) / std::max<int64_t>(items, 1) - 128);
   return p;
 }
 
-hipError_t launch_attn8_decode(const Attn8Args& a, const DecodePlan& p, int head_dim, int q_type, hipStream_t s) {
+hipError_t launch_attn8_decode(const Attn8Args& args, const DecodePlan& p, int head_dim, int q_type, hipStream_t s) {
+  Attn8Args a = args;
+  a.by_spare = divisor(p.spare);
   if (head_dim == 64) return q_type == 2 ? decode8_d<64, true>(a, p, s) : decode8_d<64, false>(a, p, s);
   if (head_dim == 96) return q_type == 2 ? decode8_d<96, true>(a, p, s) : decode8_d<96, false>(a, p, s);
   return q_type == 2 ? decode8_d<128, true>(a, p, s) : decode8_d<128, false>(a, p, s);

@@ -261,7 +261,9 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
       for (int i = 0; i < 4; ++i) bad |= !finite(o[r][d][i]);
   if (__any(bad)) pass(std::true_type{});
 
-  join_item<D, RT, NW>(a, smem, ml, last_block, m, l, o, s, sq, kvh, rb, item0, T, run, w, n, g);
+  // (a block's number is that of its run in the list)
+  const int b0 = (int)(item0 / run), b1 = (int)((item0 + T - 1) / run);
+  join_item<D, RT, NW>(a, smem, ml, last_block, m, l, o, s, sq, kvh, rb, b0, (int)blockIdx.x - b0, b1 - b0 + 1, w, n, g);
 }
 
 // Work is a list of items (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as many tiles of 32

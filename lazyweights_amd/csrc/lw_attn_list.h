@@ -1,4 +1,5 @@
-// The division of decode attention's work over blocks and the join of its parts (lw_attn_decode.hip, lw_attn8_decode.hip).
+// The division of decode attention's work over blocks (of a 16-bit cache) and the join of its parts (lw_attn_decode.hip,
+// lw_attn8_decode.hip).
 //
 // Work is a list of items (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as many tiles of KEYS
 // keys as the sequence's rows see together; the launch's blocks take equal runs of the list's tiles, whatever the lengths.
@@ -115,11 +116,13 @@ __device__ __forceinline__ void walk_items(const AttnArgs& a, uint32_t* csum, in
 
 // The end of an item's tiles in a block: the waves' maxima m, sums l of weights (each lane its own) and sums o of products (dims
 // 16 d + 4 g + i of row 16 r + n) become outputs, or this block's part of them; the block that ends an item last joins its
-// parts. Weights are of the same power of two in every wave. smem: NW [D][16] floats, done with by every wave itself; ml: [NW][RT][16][2].
+// `active` parts, of which this is number `part`. Each has a slot in the workspace, [RW] (m, l), [RW][D], two for each number from
+// base on: the first part's is 2 base + 1, part i's 2 (base + i), so that an item may begin at the number where another ends.
+// smem: NW [D][16] floats, done with by every wave itself; ml: [NW][RT][16][2].
 template <int D, int RT, int NW>
 __device__ __forceinline__ void join_item(const AttnArgs& a, uint8_t* smem, float* ml, int* last_block, const float (&m)[RT],
                                           float (&l)[RT], const f4v (&o)[RT][D / 16], int s, const Seq& sq, int kvh, int rb,
-                                          uint32_t item0, int T, uint32_t run, int w, int n, int g) {
+                                          int base_slot, int part, int active, int w, int n, int g) {
   constexpr int DT = D / 16;
   const KvView& c = a.c;
   const Divisor by_group = a.by_group;
@@ -128,10 +131,8 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, uint8_t* smem, floa
   // adds those of row x & 15, dims 4 (x >> 4) .. (and 64 on), in the waves' order.
   constexpr int RW = 16 * RT, TH = 64 * NW, Q = (4 * D + TH - 1) / TH;  // Q: groups of 4 dims per thread
   const int64_t item = ((int64_t)s * a.row_blocks + rb) * c.kv_heads + kvh;
-  const int b0 = (int)(item0 / run), b1 = (int)((item0 + T - 1) / run), active = b1 - b0 + 1;
-  // a block has two slots for its parts of items, [RW] (m, l), [RW][D]: 2 b for one that began in an earlier run, and 2 b + 1
   constexpr int SLOT = RW * (D + 2);
-  auto slot = [&](int b) { return a.part + (int64_t)(2 * b + (b == b0)) * SLOT; };
+  auto slot = [&](int i) { return a.part + (int64_t)(2 * (base_slot + i) + (i == 0)) * SLOT; };
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     l[r] = add32(add16(l[r]));
@@ -143,7 +144,7 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, uint8_t* smem, floa
   __syncthreads();
   float* ob = reinterpret_cast<float*>(smem);  // [NW waves][D / 4][16 rows][4]
   const int n2 = threadIdx.x & 15, q2 = threadIdx.x >> 4;
-  float* my_slot = slot(blockIdx.x);
+  float* my_slot = slot(part);
   auto out_at = [&](int row, int dim) {
     const int tok = by_group(row);
     return (int64_t)(sq.row0 + tok) * a.ldo + (int64_t)(kvh * a.group + row - tok * a.group) * D + dim;
@@ -214,12 +215,11 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, uint8_t* smem, floa
     float mx = -INFINITY, sum = 0.f;
     f4v acc = (f4v)0.f;
     constexpr int NB = 8;
-    for (int i0 = b0 + cg; i0 <= b1; i0 += NB * groups) {
+    for (int i0 = cg; i0 < active; i0 += NB * groups) {
       f2v h[NB], x[NB], y[NB];
 #pragma unroll
       for (int i = 0; i < NB; ++i) {  // (past the last part: the first of the turn again, with no weight)
-        const int b = i0 + i * groups <= b1 ? i0 + i * groups : i0;
-        const float* p = slot(b);
+        const float* p = slot(i0 + i * groups < active ? i0 + i * groups : i0);
         h[i] = get2(p + rr * 2);
         x[i] = get2(p + 2 * RW + rr * D + 4 * dq);
         y[i] = get2(p + 2 * RW + rr * D + 4 * dq + 2);
@@ -233,7 +233,7 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, uint8_t* smem, floa
       acc *= down;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
-        if (i0 + i * groups <= b1) {
+        if (i0 + i * groups < active) {
           const float f = pow2(h[i][0] - base);
           sum += h[i][1] * f;
           acc += (f4v){x[i][0], x[i][1], y[i][0], y[i][1]} * f;

@@ -1,4 +1,4 @@
-// Appending to a paged key-value cache held in 8 bits, and attention over it.
+// Appending to a paged key-value cache held in 8 bits.
 #include <algorithm>
 
 #include "lw_attn8_device.h"
@@ -31,8 +31,6 @@ __device__ __forceinline__ void rotate(f4v& x, f4v& y, f4v c, f4v n, bool neighb
   x = neighbours ? (f4v){t[0], w[0], t[1], w[1]} : t;
   y = neighbours ? (f4v){t[2], w[2], t[3], w[3]} : w;
 }
-
-// ── append ──────────────────────────────────────────────────────────────────────────────────────────────────────────
 
 // As k_kv_append, with keys and values quantized: a block of 2 D threads has the 16 rows that share an exponent, of the keys or
 // the values of a head, a thread 8 elements of a row: the largest magnitude of the new rows gives the exponent, and rows from
@@ -133,77 +131,6 @@ __global__ __launch_bounds__(2 * D) void k_kv8_append(const Append8Args args, ui
   }
 }
 
-// ── attention ───────────────────────────────────────────────────────────────────────────────────────────────────────
-
-// A block per (row, head): 256 keys at a time, a key per thread for the scores, then dims over threads for the sums.
-template <int D, bool BF>
-__global__ __launch_bounds__(256) void k_attn8(const Attn8Args args) {
-  constexpr int G = 256 / D;
-  const AttnArgs& a = args.a;
-  const KvView& c = a.c;
-  __shared__ float ql[D], pl[256], red[4], sums[G * D];
-  __shared__ int64_t vl[256];
-  const int row = blockIdx.x / a.heads, head = blockIdx.x - row * a.heads, kvh = a.by_group(head), t = threadIdx.x;
-  const int s = last_at_most(c.seqs, row, [&](int i) { return c.q_start[i]; });
-  const Seq sq = sequence(c, s);
-  if (row < sq.row0 || row >= sq.row0 + sq.rows) return;
-  const int pos = sq.len - sq.rows + row - sq.row0, hi = min(pos + 1, sq.len), lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
-  if (t < D) {
-    const uint16_t q = a.q[a.ldq * row + head * D + t] ^ (uint16_t)a.q_flip;
-    ql[t] = wide<BF>(q) * a.scale;
-  }
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  for (int k0 = lo; k0 < hi; k0 += 256) {
-    const int key = min(k0 + t, hi - 1), mask = (1 << c.page_shift) - 1;
-    const uint32_t page = (uint32_t)c.table[s * c.tstride + (key >> c.page_shift)];
-    const bool seen = k0 + t < hi && page < c.pages;
-    const int64_t at = (seen ? page * c.pstride : 0) + kvh * c.hstride + (key & mask) * c.rstride;
-    const int64_t eat = (seen ? page * args.e.pstride : 0) + kvh * args.e.hstride + (key & mask) / kExpBlock;
-    float x = 0.f;
-    const uint8_t* k = reinterpret_cast<const uint8_t*>(c.k) + at;
-    for (int d = 0; d < D; d += 4) {
-      const f4v v = from8(*reinterpret_cast<const uint32_t*>(k + d));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x += v[i] * ql[d + i];
-    }
-    x = seen ? x * two_to(exponent(args.e.k[eat])) : -INFINITY;
-    float mx = x;
-#pragma unroll
-    for (int d = 32; d; d /= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
-    __syncthreads();
-    if ((t & 63) == 0) red[t >> 6] = mx;
-    vl[t] = at;
-    __syncthreads();
-    mx = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-    const float base = mx == -INFINITY ? 0.f : mx, down = pow2(m - base), p = pow2(x - base);
-    m = mx;
-    pl[t] = seen ? p * two_to(exponent(args.e.v[eat])) : -1.f;
-    float sum = seen ? p : 0.f;
-#pragma unroll
-    for (int d = 32; d; d /= 2) sum += __shfl_xor(sum, d);
-    __syncthreads();
-    if ((t & 63) == 0) red[t >> 6] = sum;
-    __syncthreads();
-    l = l * down + red[0] + red[1] + red[2] + red[3];
-    o *= down;
-    if (t < G * D)
-      for (int j = t / D; j < min(256, hi - k0); j += G)
-        if (pl[j] >= 0.f || pl[j] != pl[j]) {
-          const uint8_t v = reinterpret_cast<const uint8_t*>(c.v)[vl[j] + t % D];
-          o += pl[j] * __builtin_amdgcn_cvt_f32_fp8((int)v, 0);
-        }
-  }
-  __syncthreads();
-  if (t < G * D) sums[t] = o;
-  __syncthreads();
-  if (4 * t < D) {
-    f4v v = (f4v)0.f;
-    for (int g = 0; g < G; ++g) v += *reinterpret_cast<const f4v*>(sums + g * D + 4 * t);
-    store4(a.out_type, a.out, a.ldo * row + head * D + 4 * t, normal(v, l));
-  }
-}
-
 template <int D, int X>
 hipError_t append8_d(const Append8Args& a, int q_type, hipStream_t s) {
   const uint32_t items = (uint32_t)(a.a.c.tokens / kExpBlock + 2 * a.a.c.seqs), kv_blocks = items * 2 * (uint32_t)a.a.c.kv_heads;
@@ -217,26 +144,12 @@ hipError_t append8_x(const Append8Args& a, int q_type, int x_type, hipStream_t s
   return x_type == 0 ? append8_d<D, 0>(a, q_type, s) : x_type == 1 ? append8_d<D, 1>(a, q_type, s) : append8_d<D, 2>(a, q_type, s);
 }
 
-template <int D>
-hipError_t attn8_d(const Attn8Args& a, int q_type, hipStream_t s) {
-  const dim3 grid((uint32_t)a.a.c.tokens * (uint32_t)a.a.heads);
-  if (q_type == 2) k_attn8<D, true><<<grid, 256, 0, s>>>(a);
-  else k_attn8<D, false><<<grid, 256, 0, s>>>(a);
-  return hipGetLastError();
-}
-
 }  // namespace
 
 hipError_t launch_append8(const Append8Args& a, int head_dim, int q_type, int x_type, hipStream_t s) {
   if (head_dim == 64) return append8_x<64>(a, q_type, x_type, s);
   if (head_dim == 96) return append8_x<96>(a, q_type, x_type, s);
   return append8_x<128>(a, q_type, x_type, s);
-}
-
-hipError_t launch_attn8(const Attn8Args& a, int head_dim, int q_type, hipStream_t s) {
-  if (head_dim == 64) return attn8_d<64>(a, q_type, s);
-  if (head_dim == 96) return attn8_d<96>(a, q_type, s);
-  return attn8_d<128>(a, q_type, s);
 }
 
 }  // namespace lw
