@@ -86,7 +86,7 @@ DecodePlan decode8_plan(int seqs, int kv_heads, int group, int head_dim, int max
 constexpr int kPromptSlots = 512, kLongRun = 16384;
 int64_t prompt_items(int seqs, int kv_heads, int group, int tokens);
 size_t prompt_slot_bytes(int head_dim);
-int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots);
+int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots, int least);
 
 // A cache in 8 bits: KvView's k and v are of bytes, its strides in bytes, and each 16 rows of a head have an exponent at
 // k (v) + page * pstride + head * hstride + row / 16.

@@ -181,8 +181,8 @@ bool take_plan(const char* fn, const lw::DecodePlan& p, const lw_batch* batch, l
 }
 
 // into how many blocks a prompt's row tiles share out their keys, with the workspace past `skip` (the counters of the decode call, if the
-// batch may go there)
-bool share_keys(const char* fn, const lw_batch* batch, int kv_heads, int head_dim, size_t skip, lw::AttnArgs& a) {
+// batch may go there); `least` blocks or one
+bool share_keys(const char* fn, const lw_batch* batch, int kv_heads, int head_dim, size_t skip, int least, lw::AttnArgs& a) {
   if (((long long)batch->tokens * a.group / 128 + batch->seqs) * kv_heads > kMostBlocks)
     return refuse(fn, "more tokens than a launch can take"), false;
   if (batch->workspace && (reinterpret_cast<uintptr_t>(batch->workspace) & 15)) return refuse(fn, "workspace not aligned to 16"), false;
@@ -191,7 +191,7 @@ bool share_keys(const char* fn, const lw_batch* batch, int kv_heads, int head_di
     const long long bytes = batch->workspace_bytes - (long long)skip;
     if (bytes > 0)
       a.splits = lw::prompt_splits(batch->seqs, kv_heads, a.group, batch->tokens, batch->max_kv,
-                                   bytes / (long long)lw::prompt_slot_bytes(head_dim));
+                                   bytes / (long long)lw::prompt_slot_bytes(head_dim), least);
   }
   const int most_kv = a.window > 0 ? std::min(batch->max_kv, a.window) : batch->max_kv;
   a.most_run = most_kv / a.splits;
@@ -220,7 +220,7 @@ int attend8(const char* fn, bool decode, const lw_kv8_cache* cache, const lw_bat
   if (batch->max_new <= 16)
     skip = lw::decode8_plan(batch->seqs, cache->kv_heads, a.a.group, cache->head_dim, std::max(batch->max_new, 1), batch->max_kv)
                .count_bytes;
-  if (!share_keys(fn, batch, cache->kv_heads, cache->head_dim, skip, a.a)) return -1;
+  if (!share_keys(fn, batch, cache->kv_heads, cache->head_dim, skip, 2, a.a)) return -1;
   return launched(fn, lw::launch_attn8_prompt(a, cache->head_dim, q_type, static_cast<hipStream_t>(stream)));
 }
 
@@ -275,7 +275,7 @@ int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
   if (batch->max_new <= 16)
     skip = lw::decode_plan(batch->seqs, cache->kv_heads, a.group, cache->head_dim, std::max(batch->max_new, 1), batch->max_kv)
                .count_bytes;
-  if (!share_keys(fn, batch, cache->kv_heads, cache->head_dim, skip, a)) return -1;
+  if (!share_keys(fn, batch, cache->kv_heads, cache->head_dim, skip, 3, a)) return -1;
   return launched(fn, lw::launch_attn_prompt(a, cache->head_dim, cache->type, static_cast<hipStream_t>(stream)));
 }
 
@@ -283,8 +283,8 @@ long long lw_attn8_workspace(const lw_kv8_cache* cache, const lw_batch* batch, i
   const std::string bad = check8(cache, batch, heads);
   if (!bad.empty()) return refuse("lw_attn8_workspace", bad);
   if (batch->seqs == 0) return 0;
-  if (batch->max_new > 16)
-    return batch->max_kv < 3 * 1024 ? 0 : (long long)(lw::kPromptSlots * lw::prompt_slot_bytes(cache->head_dim));
+  if (batch->max_new > 16)  // (a row tile's keys are shared out where there are twice 1024 and more)
+    return batch->max_kv < 2 * 1024 ? 0 : (long long)(lw::kPromptSlots * lw::prompt_slot_bytes(cache->head_dim));
   const lw::DecodePlan p = lw::decode8_plan(batch->seqs, cache->kv_heads, heads / cache->kv_heads, cache->head_dim, batch->max_new,
                                             batch->max_kv);
   return (long long)(p.count_bytes + p.part_bytes);

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
 #pragma unroll
   for (int i = 0; i < 2 * C; ++i) qf[i] = *reinterpret_cast<const u32x4*>(q_from + 16 * i) ^ flip;
 
-  const int lrow = F8 ? lane & 15 : ((lane & 15) - 4 * (lane >> 4)) & 15;  // the row of its block that this lane copies
+  const int lrow = ((lane & 15) - 4 * (lane >> 4)) & 15;  // the row of its block that this lane copies
   const int32_t* table = c.table + s * c.tstride;
   const uint16_t* kb = c.k + kvh * c.hstride + 8 * (lane >> 4);
   const uint16_t* vb = c.v + kvh * c.hstride + 8 * (lane >> 4);
@@ -136,34 +136,45 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
   auto ask_page = [&](int t) { pg = (uint32_t)table[key_of(t) >> c.page_shift]; };
   // a wave's share of a tile's copy, in PIECES instructions of 1 KB: where from, then piece by piece (a run of them would
   // keep every wave waiting for the address units at the start of a tile)
-  // (of 8 bits: 16 bytes of a row, 8 the last of 96)
-  constexpr int EACH = F8 ? (C + 1) / 2 : C, PIECES = W == 4 ? 2 * EACH : EACH;
+  // (of 8 bits: keys 8 u .. 8 u + 7 of K and of V for each unit u = w, and w + 4 of 4 waves, a lane 16 bytes of row lane & 7)
+  constexpr int UNITS = 8 / W, PIECES = F8 ? 2 * UNITS : W == 4 ? 2 * C : C;
   const uint16_t *k_from = nullptr, *v_from = nullptr;
-  u32x4 raw[F8 ? PIECES : 1];
-  int raw_e[2] = {0, 0};
-  uint64_t raw_there = 0;
-  // 8 bits: a wave's share of tile t on its way
-  auto load = [&](int t) {
-    if constexpr (F8) {
-      bool there;
-      const int key = key_of(t);
-      const int64_t off = key_offset(c, pg, key, there) + kvh * c.hstride;
-      const int64_t eoff = (there ? pg * args.e.pstride : 0) + kvh * args.e.hstride + (key & ((1 << c.page_shift) - 1)) / kExpBlock;
-      raw_there = __ballot(there);
-      if (W == 4 || w < 4) raw_e[0] = args.e.k[eoff];
-      if (W == 4 || w >= 4) raw_e[1] = args.e.v[eoff];
+  // where a lane's 16 bytes go, two chunks
+  int put_at[2];
 #pragma unroll
-      for (int j = 0; j < PIECES; ++j) {
-        const bool key_piece = W == 4 ? j < EACH : w < 4;
-        const uint8_t* from = reinterpret_cast<const uint8_t*>(key_piece ? c.k : c.v) + off;
-        if (C % 2 && j % EACH == EACH - 1) {
-          const uint2 u = *reinterpret_cast<const uint2*>(from + 64 * (j % EACH) + 8 * (lane >> 4));
-          raw[j] = (u32x4){u.x, u.y, 0, 0};
-        } else {
-          raw[j] = *reinterpret_cast<const u32x4*>(from + 64 * (j % EACH) + 16 * (lane >> 4));
-        }
-      }
+  for (int i = 0; i < 2; ++i) {
+    const int ch = 2 * (lane >> 3) + i, row = 8 * (w & 1) + (lane & 7);
+    put_at[i] = 2 * ((w >> 1) * BLK + ch * 128 + ((row + 4 * ch) & 15) * 8);
+  }
+  u32x4 raw[F8 ? PIECES : 1];
+  int raw_e[F8 ? PIECES : 1];
+  uint32_t raw_pg[UNITS];
+  bool raw_there[UNITS];
+  // the first key of a unit of tile t (past the last key: of the unit that holds it)
+  auto unit_key = [&](int t, int u) { return min(lo + 64 * t + 8 * (w + 4 * u), (hi - 1) & ~7); };
+  auto ask_pages = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) raw_pg[u] = (uint32_t)table[unit_key(t, u) >> c.page_shift];
+  };
+  // unit u of tile t on its way
+  auto load_unit = [&](int t, int u) {
+    if constexpr (F8) {
+      const uint32_t page = __builtin_amdgcn_readfirstlane(raw_pg[u]);
+      const int key = unit_key(t, u), in_page = key & ((1 << c.page_shift) - 1);
+      raw_there[u] = page < c.pages;
+      const int64_t at = raw_there[u] ? page : 0;
+      const int64_t off = at * c.pstride + kvh * c.hstride + (int64_t)in_page * c.rstride;
+      const int64_t eoff = at * args.e.pstride + kvh * args.e.hstride + in_page / kExpBlock;
+      const uint32_t mine = (uint32_t)min(lane & 7, hi - 1 - key) * (uint32_t)c.rstride + 16 * min(lane >> 3, D / 16 - 1);
+      raw[2 * u] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(c.k) + off + mine);
+      raw[2 * u + 1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(c.v) + off + mine);
+      raw_e[2 * u] = args.e.k[eoff];
+      raw_e[2 * u + 1] = args.e.v[eoff];
     }
+  };
+  auto load = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) load_unit(t, u);
   };
   auto locate = [&](int t) {
     bool there;
@@ -176,34 +187,31 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
   // (t: the tile that is worked on, the one before the piece's)
   auto piece = [&](int j, uint16_t* kt, uint16_t* vt, int t) {
     if constexpr (F8) {
-      const bool key_piece = W == 4 ? j < EACH : w < 4;
-      uint16_t* to = (key_piece ? kt : vt) + wb * BLK;
-      auto put = [&](int ch, uint32_t x, uint32_t y) {
-        const u32x4 v = key_piece ? widen8<BF>(x, y) : widen8<false>(x, y);
-        *reinterpret_cast<u32x4*>(to + ch * 128 + ((lrow + 4 * ch) & 15) * 8) = v;
-      };
-      if (C % 2 && j % EACH == EACH - 1) {
-        put(8 * (j % EACH) + (lane >> 4), raw[j][0], raw[j][1]);
+      const int u = j >> 1, block = (w >> 1) + 2 * u;
+      uint16_t* to = (j & 1 ? vt : kt) + 2 * u * BLK;
+      asm("" : "+v"(put_at[0]), "+v"(put_at[1]));  // (or the compiler keeps the address in every buffer)
+      if (D == 128 || (lane >> 3) < D / 16)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          *reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(to) + put_at[i]) =
+              j & 1 ? widen8<false>(raw[j][2 * i], raw[j][2 * i + 1]) : widen8<BF>(raw[j][2 * i], raw[j][2 * i + 1]);
+      // (the same values from every lane, and from the two units of a block)
+      const int to_tile = (t + 1) & 1, e = clampi(raw_e[j], -kMostExp, kMostExp);
+      if (j & 1) {
+        ve_l[to_tile][block] = (float)e;
+        iv_l[to_tile][block] = two_to(-e);
       } else {
-        put(8 * (j % EACH) + 2 * (lane >> 4), raw[j][0], raw[j][1]);
-        put(8 * (j % EACH) + 2 * (lane >> 4) + 1, raw[j][2], raw[j][3]);
-      }
-      if (j == 0 && lane == 0) {
-        const int b = (t + 1) & 1;
-        if (W == 4 || w < 4) {
-          seen_l[b][wb] = raw_there & 1 ? 0xFFFF : 0;
-          ks_l[b][wb] = fmaxf(a.scale * two_to(clampi(raw_e[0], -kMostExp, kMostExp)), 1e-37f);
-        }
-        if (W == 4 || w >= 4) {
-          const int e = clampi(raw_e[1], -kMostExp, kMostExp);
-          ve_l[b][wb] = (float)e;
-          iv_l[b][wb] = two_to(-e);
-        }
+        seen_l[to_tile][block] = raw_there[u] ? 0xFFFF : 0;
+        ks_l[to_tile][block] = fmaxf(a.scale * two_to(e), 1e-37f);
       }
       return;
     }
     if (W == 4 ? j < C : w < 4) copy_lds16(k_from + 32 * (j % C), kt + wb * BLK + 512 * (j % C));
     else copy_lds16(v_from + 32 * (j % C), vt + wb * BLK + 512 * (j % C));
+  };
+  // (offsets in bytes of 8 bits)
+  auto in_tile = [](const uint16_t* buf, int at) {
+    return F8 ? reinterpret_cast<const uint16_t*>(reinterpret_cast<const uint8_t*>(buf) + at) : buf + at;
   };
   // where a lane reads: K, chunk 2 i + g of key n & 15 of block 2 h + (n >> 4), by the parity of i; V, 4 dims of chunk
   // 4 d + c0 of key 8 e + 4 g + (lane >> 2 & 3) of block q
@@ -211,8 +219,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
   int kr[2], vr[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    kr[i] = (n >> 4) * BLK + g * 128 + (((n & 15) + 8 * i + 4 * g) & 15) * 8;
-    vr[i] = c0 * 128 + ((8 * i + 4 * g + ((lane >> 2) & 3) + 4 * c0) & 15) * 8 + 4 * (lane & 1);
+    kr[i] = (F8 ? 2 : 1) * ((n >> 4) * BLK + g * 128 + (((n & 15) + 8 * i + 4 * g) & 15) * 8);
+    vr[i] = (F8 ? 2 : 1) * (c0 * 128 + ((8 * i + 4 * g + ((lane >> 2) & 3) + 4 * c0) & 15) * 8 + 4 * (lane & 1));
   }
 
   float m, l, lost;  // lost: what rounding has added to l
@@ -233,12 +241,13 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
     auto scores = [&](int t, const uint16_t* buf, auto between) {
       const int t0 = lo + 64 * t;
       f16x16 sc[2];
+      if (F8 && W == 4) asm("" : "+v"(kr[0]), "+v"(kr[1]));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         sc[h] = (f16x16)0.f;
 #pragma unroll
         for (int i = 0; i < 2 * C; ++i) {
-          sc[h] = mfma32<BF>(*reinterpret_cast<const u32x4*>(buf + kr[i & 1] + 2 * h * BLK + 256 * i), qf[i], sc[h]);
+          sc[h] = mfma32<BF>(*reinterpret_cast<const u32x4*>(in_tile(buf, kr[i & 1]) + 2 * h * BLK + 256 * i), qf[i], sc[h]);
           between(2 * C * h + i);
         }
       }
@@ -310,13 +319,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
       u32x4 vt;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const uint2 u = read_tr(buf + vr[e] + q * BLK + 512 * d);
+        const uint2 u = read_tr(in_tile(buf, vr[e]) + q * BLK + 512 * d);
         vt[2 * e] = u.x;
         vt[2 * e + 1] = u.y;
       }
       return vt;
     };
-    auto values = [&](const uint16_t* buf) {
+    auto values_with = [&](const uint16_t* buf, auto between) {
+      if (F8 && W == 4) asm("" : "+v"(vr[0]), "+v"(vr[1]));
       if constexpr (LONG && !CAREFUL) {
 #pragma unroll
         for (int d = 0; d < C; ++d) {
@@ -329,6 +339,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
           }
           o[d] += t;
         }
+        for (int q = 0; q < 4; ++q) between(q);
         return;
       }
 #pragma unroll
@@ -359,8 +370,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
             for (int i = 0; i < NP; ++i) o[d] = mfma32<VBF>(vt, part[q][i], o[d]);
           }
         }
+        between(q);
       }
     };
+    auto values = [&](const uint16_t* buf) { values_with(buf, [](int) {}); };
     auto ask = [&](int t) {  // (the last tile is copied twice: no branch between the products)
       if (F8) return;
       locate(min(t + 1, tiles - 1));
@@ -369,7 +382,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
     auto ask_after = [&](int t) {  // 8 bits: when the next tile is out of the registers
       if (!F8) return;
       load(min(t + 2, tiles - 1));
-      ask_page(min(t + 3, tiles - 1));
+      ask_pages(min(t + 3, tiles - 1));
     };
     auto step = [&](int t, const uint16_t* kt, uint16_t* k_next, uint16_t* v_next) {
       constexpr int EVERY = 4 * C / PIECES;
@@ -402,34 +415,48 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
     };
     // the same with four buffers of V, and the tiles before and after those that its rows see in loops of their own: a branch
     // around the products has their sums moved from register to register (15999 tokens 2070 us against 2140 then; of two buffers
-    // the branch is up to 3 % faster)
+    // the branch is up to 3 % faster, but of 8 bits leaves too few registers)
     auto run4 = [&] {
       auto copies = [&](int t, int end) {
         for (; t < end; ++t) {
           ask(t);
           const int b = (t + 1) & 3;
-          only_copy(t, t & 1 ? k0 : k1, b == 0 ? v0 : b == 1 ? v1 : b == 2 ? v2 : v3);
+          if constexpr (W == 8) only_copy(t, t & 1 ? k0 : k1, b == 0 ? v0 : b == 1 ? v1 : b == 2 ? v2 : v3);
+          else only_copy(t, t & 1 ? k0 : k1, t & 1 ? v0 : v1);
           arrived<F8>();
         }
       };
       auto one = [&](int t, const uint16_t* kt, const uint16_t* vt, uint16_t* k_next, uint16_t* v_next) {
         ask(t);
-        step(t, kt, k_next, v_next);
-        values(vt);
+        if constexpr (F8 && W == 4) {  // (beside the first product there are no registers for the next tile's way)
+          scores(t, kt, [](int) {});
+          values_with(vt, [&](int q) {
+            piece(q, k_next, v_next, t);
+            if (q & 1) load_unit(min(t + 2, tiles - 1), q >> 1);
+            if (q == 3) ask_pages(min(t + 3, tiles - 1));
+          });
+        } else {
+          step(t, kt, k_next, v_next);
+          values(vt);
+        }
         arrived<F8>();
       };
-      // (from a multiple of four on: what is seen of the tiles up to three before is masked)
+      // (from a multiple of the buffers on: what is seen of the tiles up to three before is masked)
       const int end = empty ? 0 : max(min((whi - lo + 64) >> 6, tiles), 0);
-      int t = a.window > 0 ? min(max((wlo - a.window - lo + 1) >> 6, 0) & ~3, end) : 0;
+      int t = a.window > 0 ? min(max((wlo - a.window - lo + 1) >> 6, 0) & (W == 8 ? ~3 : ~1), end) : 0;
       copies(0, t);
       while (t < end) {
         one(t, k0, v0, k1, v1);
         if (++t == end) break;
-        one(t, k1, v1, k0, v2);
-        if (++t == end) break;
-        one(t, k0, v2, k1, v3);
-        if (++t == end) break;
-        one(t, k1, v3, k0, v0);
+        if constexpr (W == 8) {
+          one(t, k1, v1, k0, v2);
+          if (++t == end) break;
+          one(t, k0, v2, k1, v3);
+          if (++t == end) break;
+          one(t, k1, v3, k0, v0);
+        } else {
+          one(t, k1, v1, k0, v0);
+        }
         ++t;
       }
       copies(t, tiles);
@@ -454,18 +481,22 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
         values(b == 0 ? v0 : b == 1 ? v1 : b == 2 ? v2 : v3);
       }
     };
-    ask_page(0);
-    if (F8) load(0);
-    else locate(0);
-    if (F8) ask_page(min(1, tiles - 1));
+    if (F8) {
+      ask_pages(0);
+      load(0);
+      ask_pages(min(1, tiles - 1));
+    } else {
+      ask_page(0);
+      locate(0);
+    }
 #pragma unroll
     for (int j = 0; j < PIECES; ++j) piece(j, k0, v0, -1);
     if (F8) ask_after(-1);
     else ask_page(min(1, tiles - 1));
     arrived<F8>();
-    if constexpr (W == 4) {
+    if constexpr (W == 4 && !F8) {
       run();
-    } else if constexpr (CAREFUL) {
+    } else if constexpr (W == 4 || CAREFUL) {
       run4();
     } else {
       if (w < 4) run4();

@@ -41,13 +41,14 @@ int64_t prompt_items(int seqs, int kv_heads, int group, int tokens) {
 
 size_t prompt_slot_bytes(int head_dim) { return (size_t)128 * (head_dim + 4) * 4; }
 
-int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots) {
-  // Two blocks per CU, of 1024 keys and more, where that makes three at least of every row tile's: us with / without, the join
+int prompt_splits(int seqs, int kv_heads, int group, int tokens, int max_kv, int64_t slots, int least) {
+  // Two blocks per CU, of 1024 keys and more, where that makes `least` at least of every row tile's, three of 16 bits: us with / without, the join
   // included, 64 tokens after 20000 59 / 504, 500 after 3000 52 / 89; two shares of 256 row tiles gain nothing (1000 tokens
-  // after 9001 100 / 106, their sums' way through memory takes 13), nor do few keys (700 tokens 27 / 25).
+  // after 9001 100 / 106, their sums' way through memory takes 13), nor do few keys (700 tokens 27 / 25). Of 8 bits, whose tiles pass through registers and are longer on their way, two do:
+  // the same 103 / 127.
   const int64_t items = prompt_items(seqs, kv_heads, group, tokens);
   const int64_t splits = std::min<int64_t>(std::min<int64_t>(kPromptSlots, slots) / items, max_kv / 1024);
-  return splits < 3 ? 1 : (int)splits;
+  return splits < least ? 1 : (int)splits;
 }
 
 hipError_t launch_attn_prompt(const AttnArgs& a, int head_dim, int type, hipStream_t s) {
