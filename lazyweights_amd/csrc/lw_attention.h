@@ -74,7 +74,9 @@ struct AttnArgs {
 struct DecodePlan {
   int row_tiles, row_blocks, blocks, blocks_log2, most_keys;
   bool whole;  // a block per item (of 16 bits: of 8 waves)
-  int spare;   // (8 bits) blocks beyond one for every item
+  // (8 bits) blocks have equal runs of the list, or a part of an item each: as many as items and `spare`
+  bool runs;
+  int spare, waves;
   size_t count_bytes, part_bytes;  // workspace: counters (zero before and after a launch), then partials
 };
 DecodePlan decode_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv);

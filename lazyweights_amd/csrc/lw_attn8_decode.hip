@@ -8,12 +8,15 @@ namespace lw {
 
 namespace {
 
+// LDS of a wave: its V tile and the weights of 32 keys, then [D][16] sums
+constexpr int decode8_wave(int dim, int blocks) { return std::max(16 * blocks * dim + 32 * 16 * 4, 64 * dim); }
+
 // The part of an item that a block has. Items are (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as
-// many tiles of KEYS keys as the sequence's rows see together. Of a list of all items' tiles a part takes `run` at most, total /
-// spare, so that items + spare blocks are enough whatever the lengths; parts of one item alone, so that a block has one pass, one
-// join and is done, and what it waits for in turn is covered by the blocks beside it. (Equal runs of the list for a block
-// per place on the card, as for 16 bits, have a block go from item to item, each waited for anew: us with runs / parts, 256 sequences of
-// 100-2000 keys, 8 heads of 128: 119 / 91, 30 of them 29 / 19, one of 30000 26 / 20.)
+// many tiles of KEYS keys as the sequence's rows see together. A part takes `run` tiles at most, the tiles of all items / spare, so that
+// items + spare blocks are enough whatever the lengths; parts are of one item alone, so that a block has one pass, one join and is
+// done, and what it waits for in turn is covered by the blocks beside it. (With equal runs of the list of all items a block goes
+// from item to item, each waited for anew: us with runs / parts, 256 sequences of 100-2000 keys, 8 heads of 128: 119 / 91, 30 of
+// them 29 / 19, one of 30000 26 / 20.)
 struct Part {
   Seq sq;
   int s, kvh, rb, lo, t_from, t_to;
@@ -128,21 +131,13 @@ __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles
 }
 
 template <int D, bool BF, int RT, int NW, int H>
-__global__ __launch_bounds__(64 * NW, RT == 1 ? 4 : 2) void k_attn8_decode(const Attn8Args args) {
+__device__ __forceinline__ void decode8_part(const Attn8Args& args, uint8_t* smem, float* ml, int* last_block, const Part& p0, int lane,
+                                             int w, int n, int g) {
   constexpr int KEYS = 16 * H, C = D / 32, DT = D / 16, NP = 2, FULL = D / 64, TAIL = C % 2;
   constexpr float LIFT = lift<false>(0);
-  // the waves' V tiles, and behind each the weights of 32 keys of the careful pass (after the loop their sums); then, of more than one
-  // row tile, q
-  constexpr int WAVE = std::max(KEYS * D + 32 * 16 * 4, 64 * D);
-  __shared__ __align__(16) uint8_t smem[NW * WAVE + (RT > 1 ? NW * RT * 16 * D * 2 : 0)];
-  __shared__ float ml[NW * 16 * RT * 2];
-  __shared__ int last_block;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  constexpr int WAVE = decode8_wave(D, H);
   const AttnArgs& a = args.a;
   const KvView& c = a.c;
-  Part p0;
-  uint32_t* sums_l = reinterpret_cast<uint32_t*>(smem);  // of tiles and of parts of the sequences up to each 64th
-  if (!find_part<NW, KEYS>(args, sums_l, sums_l + 1024, lane, w, p0)) return;
   const Seq& sq = p0.sq;
   const int s = p0.s, kvh = p0.kvh, rb = p0.rb, lo = p0.lo, t_from = p0.t_from, t_to = p0.t_to;
   const Divisor by_group = a.by_group;
@@ -350,14 +345,55 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 4 : 2) void k_attn8_decode(const
       for (int i = 0; i < 4; ++i) bad |= !finite(o[r][d][i]);
   if (__any(bad)) pass(std::true_type{});
 
-  join_item<D, RT, NW>(a, smem, ml, &last_block, m, l, o, s, sq, kvh, rb, p0.base_slot, p0.part, p0.active, w, n, g);
+  join_item<D, RT, NW>(a, smem, ml, last_block, m, l, o, s, sq, kvh, rb, p0.base_slot, p0.part, p0.active, w, n, g);
+}
+
+// Attention over 8 bits: scores S^T = K Q^T of 16 rows and 32 keys of each wave's tiles, O^T = V^T P^T, numbers made 16 bits of
+// q's type (K) and fp16 (V) in registers, where both are exact: an instruction for two numbers, at the full rate. K's power of two is a
+// factor of a block's scores; V's enters the weight, 2^(score + e - m) with m the largest score + e, so that weights need no more range
+// than before, and the sum of weights takes it off again by the block. Bytes of V go to LDS as they are and come back transposed
+// (ds_read_b64_tr_b8), eight keys of a dim per lane.
+//
+// Bound by memory: 2 D + 1/8 bytes a key and key-value head. A wave has a tile of 32 keys (8 KB at D = 128) on its way while it works on the
+// one before; 128 registers leave room for 16 waves a CU (64 keys a tile and 8 waves: 64 sequences of 500-16000 keys 127 us against
+// 123, 256 of 100-2000 94 against 91). us, and of the bytes: 64 sequences of 500-16000 keys, 8 heads of 128: 123 (580 MB: 4.7
+// TB/s); one of 131071: 55 (268 MB: 4.9, 5.4 in the loop); 4 x 5 tokens of 32 heads of 96 over 301-5003: 11.7 (50 MB); one of 778: 8.2.
+// A launch without its bytes is 6 us (200 keys: 6.7): start, lengths 1, page and first tile 1.5, stores of a part until they are
+// counted 2; the last part's join 2 to 4 more.
+//
+// RUNS: a block has an equal run of the list of all items' tiles (walk_items) instead of a part.
+template <int D, bool BF, int RT, int NW, int H, bool RUNS>
+__global__ __launch_bounds__(64 * NW, RT == 1 && !RUNS ? 4 : 2) void k_attn8_decode(const Attn8Args args) {
+  // the waves' V tiles, and behind each the weights of 32 keys of the careful pass (after the loop their sums); then, of more than one
+  // row tile, q
+  __shared__ __align__(16) uint8_t smem[NW * decode8_wave(D, H) + (RT > 1 ? NW * RT * 16 * D * 2 : 0)];
+  __shared__ float ml[NW * 16 * RT * 2];
+  __shared__ uint32_t csum[RUNS ? 1024 : 1];
+  __shared__ int last_block;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+  if constexpr (RUNS) {
+    walk_items<NW, 16 * H>(args.a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0,
+                                                      int T, uint32_t run) __attribute__((always_inline)) {
+      // (a block's number is that of its run in the list)
+      const int b0 = (int)(item0 / run), b1 = (int)((item0 + T - 1) / run);
+      const Part p = {sq, s, kvh, rb, lo, t_from, t_to, b0, (int)blockIdx.x - b0, b1 - b0 + 1};
+      decode8_part<D, BF, RT, NW, H>(args, smem, ml, &last_block, p, lane, w, n, g);
+    });
+  } else {
+    Part p;
+    uint32_t* sums_l = reinterpret_cast<uint32_t*>(smem);  // of tiles and of parts of the sequences up to each 64th
+    if (find_part<NW, 16 * H>(args, sums_l, sums_l + 1024, lane, w, p))
+      decode8_part<D, BF, RT, NW, H>(args, smem, ml, &last_block, p, lane, w, n, g);
+  }
 }
 
 template <int D, bool BF>
 hipError_t decode8_d(const Attn8Args& a, const DecodePlan& p, hipStream_t s) {
   const dim3 grid((uint32_t)p.blocks);
-  if (p.row_tiles == 1) k_attn8_decode<D, BF, 1, 4, 2><<<grid, 256, 0, s>>>(a);
-  else k_attn8_decode<D, BF, 2, 4, 2><<<grid, 256, 0, s>>>(a);
+  if (p.row_tiles == 2) k_attn8_decode<D, BF, 2, 4, 2, false><<<grid, 256, 0, s>>>(a);
+  else if (D == 128 && p.runs) k_attn8_decode<128, BF, 1, 4, 2, true><<<grid, 256, 0, s>>>(a);
+  else if (p.waves == 8) k_attn8_decode<D, BF, 1, 8, 2, false><<<grid, 512, 0, s>>>(a);
+  else k_attn8_decode<D, BF, 1, 4, 2, false><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 
@@ -366,18 +402,36 @@ hipError_t decode8_d(const Attn8Args& a, const DecodePlan& p, hipStream_t s) {
 DecodePlan decode8_plan(int seqs, int kv_heads, int group, int head_dim, int max_new, int max_kv) {
   DecodePlan p;
   const int rows = group * max_new;
+  // Two row tiles per item share what is read, where there is much to read (us with two / one: 8 sequences of 1000-8000 keys, 8 heads of
+  // 128, 20 rows 29 / 34, 64 of 500-16000 194 / 242; one of 500, 64 rows 15 / 10, 4 of 300-5000 23 / 22).
   p.row_tiles = rows <= 16 || (int64_t)seqs * kv_heads * max_kv < 1 << 18 ? 1 : 2;
   p.row_blocks = (rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles);
   const int64_t items = (int64_t)seqs * kv_heads * p.row_blocks, tiles = items * (max_kv / 32 + 2);
+  // A block per item, which has nothing to find out and nothing to join: where an item is one or two tiles for each wave (200 keys 6.7
+  // us), and where there are many, none long (us against parts: 1024 items of 300-1000 keys 42 / 44, 2048 of 100-2000 91 / 95; 512 of
+  // two row tiles and 100-3000 keys 53 / 62; but 240 of 100-2000 20 / 18).
+  p.whole = items <= 1 << 20 && (max_kv <= 256 || (p.row_tiles == 2 ? items >= 512 && max_kv <= 4096 : items >= 1024 && max_kv <= 2048));
+  // Equal runs of the list of all items, for 512 blocks, where there are many and long ones: what a CU has to read is then the same
+  // everywhere, and a CU takes little more than its share of the card's rate (parts end unevenly, whatever their number). us with runs
+  // / parts: 512 items of 500-16000 keys 123 / 133, 1024 of them 241 / 261, 512 of 8000 189 / 207, 2048 of 300-8000 248 / 283, 256 of
+  // 500-16000 66 / 71; 512 of 300-5000 58 / 61. Heads of 96, whose tiles are smaller, need more waves beside one another: 124 / 101.
+  p.runs = !p.whole && p.row_tiles == 1 && head_dim == 128 && items >= 256 && max_kv > 4096;
+  p.blocks_log2 = 9;
+  // Parts: few items in about as many blocks as there are CUs (the more parts of an item, the longer its join: one of 131071 keys with
+  // 248 spare blocks 58 us, 504 60, 1016 82; one of 30000 19, 25, 41), some more for items that are shorter (128 of 1000-3000 keys with
+  // 248 24, 504 20); many items so that a part is of some 100 tiles at the bounds.
   const int64_t few = items <= 64 ? 256 - items : std::max<int64_t>(512 - items, 256);
   const int64_t many = std::min<int64_t>(std::max<int64_t>(tiles / 96, 512), 2048);
-  p.whole = items <= 1 << 20 && (max_kv <= 256 || (items >= 1024 && max_kv <= 2048));
-  p.blocks_log2 = 0;
   p.spare = (int)std::max<int64_t>(1, std::min<int64_t>(items > 256 ? many : few, (tiles + 3) / 4));
-  p.blocks = (int)items + (p.whole ? 0 : p.spare);
+  p.blocks = p.runs ? 1 << p.blocks_log2 : (int)items + (p.whole ? 0 : p.spare);
+  // 8 waves where one block of a CU has a long part: half as many parts would leave half of the CUs idle, and 4 waves ask for too little
+  // at a time (one of 131071 keys 55 / 58; one of 778 10.4 / 8.2)
+  p.waves = !p.whole && items <= 64 && tiles / p.spare >= 64 ? 8 : 4;
   p.count_bytes = ((size_t)items * 4 + 255) & ~(size_t)255;
-  p.part_bytes = ((size_t)p.spare + 1) * 2 * p.row_tiles * 16 * (head_dim + 2) * 4;
-  p.most_keys = (int)std::min<int64_t>(1 << 30, ((int64_t)1 << 36) / std::max<int64_t>(items, 1) - 128);
+  // (two slots for every run of the list: blocks of runs have one each, parts as many as there are spare blocks, and one begun)
+  p.part_bytes = (size_t)(p.runs ? p.blocks : p.spare + 1) * 2 * p.row_tiles * 16 * (head_dim + 2) * 4;
+  // (and 2^13 fewer, so that a run of the list of all of them, rounded up, is counted in 31 bits)
+  p.most_keys = (int)std::min<int64_t>(1 << 30, (((int64_t)1 << 36) - (1 << 18)) / std::max<int64_t>(items, 1) - 128);
   return p;
 }
 

@@ -154,6 +154,14 @@ BATCHES = [
     ((64, 2, 96), 5, 2000, 2000, 1),
     ((8, 4, 64), 1000, 3, 9000, 1),
     ((32, 1, 128), 9, 4100, 16000, 3),
+    # many items with long bounds: equal runs of the list, of up to 64 sequences and of more
+    ((32, 8, 128), 60, 900, 6000, 2),
+    ((8, 4, 128), 300, 200, 4500, 1),
+    ((16, 8, 128), 33, 5000, 5000, 1),
+    # two row tiles in a block per item, in parts
+    ((32, 4, 128), 130, 300, 600, 3),
+    ((24, 4, 64), 300, 60, 2000, 5),
+    ((20, 2, 96), 70, 700, 9000, 4),
 ]
 
 
@@ -368,6 +376,31 @@ def test_long_cache_same_bits_every_call(gpu, lib):
     kk, vv = (values(torch, *t)[table[0].long(), 0].reshape(-1, 128)[:70001] for t in ((k, k_exp), (v, v_exp)))
     ref = torch.softmax(q[0].double() @ kk.T.contiguous() * 128 ** -0.5, -1) @ vv
     assert ((first[0].double() - ref).norm() / ref.norm()).item() < 1e-5
+
+
+@pytest.mark.parametrize("window", (0, 100000))
+def test_long_parts(gpu, lib, window):
+    """One long sequence, whose parts are of blocks with 8 waves: some rows against 64 bits, NaN that only the last row sees."""
+    import torch
+    from lazyweights_amd import Batch, KvCache8
+    g = torch.Generator(device="cuda").manual_seed(32)
+    keys, kv, heads, page = 140003, 4, 16, 64
+    pages = -(-keys // page)
+    (k, k_exp), (v, v_exp) = (held(torch, torch.randn((pages, kv, page, 128), generator=g, device="cuda"), 1) for _ in range(2))
+    table = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)[None].contiguous()
+    cache = KvCache8(k, v, k_exp, v_exp)
+    batch = Batch(cache, heads, torch.tensor([0, 3], dtype=torch.int32, device="cuda"),
+                  torch.tensor([keys], dtype=torch.int32, device="cuda"), table, 3, keys)
+    q = torch.randn((3, heads, 128), generator=g, device="cuda").half()
+    v.view(torch.uint8)[int(table[0, (keys - 1) // page]), 1, (keys - 1) % page, 9] = 0x7F
+    y = cache.attend_decode(batch, q, out=torch.empty_like(q, dtype=torch.float32), window=window)
+    assert torch.isnan(y[2, 4:8, 9]).all() and int(torch.isnan(y).sum()) == 4
+    for row in range(2):
+        at = torch.arange(max(0, keys - 2 + row - window) if window else 0, keys - 2 + row, device="cuda")
+        kk, vv = (values(torch, *t)[table[0, at // page].long(), :, at % page] for t in ((k, k_exp), (v, v_exp)))
+        p = torch.softmax(torch.einsum("hgd,jhd->hgj", q[row].double().view(kv, 4, 128), kk) * 128 ** -0.5, -1)
+        ref = torch.einsum("hgj,jhd->hgd", p, vv).reshape(heads, 128)
+        assert ((y[row].double() - ref).norm() / ref.norm()).item() < 1e-5
 
 
 def test_streams_and_captured_calls(gpu, lib):
