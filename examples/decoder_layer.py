@@ -3,11 +3,12 @@ then one token per sequence and step, then a draft of a few tokens per sequence 
 
     python examples/decoder_layer.py            # a Mistral-7B-shaped layer, synthetic weights
     python examples/decoder_layer.py --small    # 512 wide
+    python examples/decoder_layer.py --cache8   # keys and values held in 8 bits
 
 The matrices (q, k, v, o, gate, up, down) are multiplied from their coded form (Runtime.matmul_dev); between q, k, v and o the
-keys and values go into a paged cache, rotated on the way, and the new tokens attend over it (KvCache, Batch). Norms and the
-gate are plain torch. Pages are handed out from a pool as sequences grow; the batch of a decode step and its tensors are kept
-over the steps, so that the loop only writes lengths and page numbers on the GPU.
+keys and values go into a paged cache, rotated on the way, and the new tokens attend over it (KvCache or KvCache8, Batch). Norms and
+the gate are plain torch. Pages are handed out on the GPU as sequences grow (Pages); the batch of a decode step and its tensors
+are kept over the steps, so that the loop only says how many tokens each sequence gets.
 """
 import argparse
 import os
@@ -19,7 +20,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 
 import torch  # noqa: E402
 
-from lazyweights_amd import Batch, KvCache, Runtime, bundle  # noqa: E402
+from lazyweights_amd import Batch, KvCache, KvCache8, Pages, Runtime, bundle  # noqa: E402
 from lazyweights_amd.configs import MISTRAL, Q4_K  # noqa: E402
 
 SMALL = [("q", 512, 512), ("k", 128, 512), ("v", 128, 512), ("o", 512, 512), ("gate", 1024, 512), ("up", 1024, 512),
@@ -32,13 +33,13 @@ def write_layer(path, shapes, seed=2000):
 
 
 class Layer:
-    """One decoder layer over a bundle, with a cache of `pages` pages that its sequences share."""
+    """One decoder layer over a bundle, with a cache of `pages` pages that its sequences share, of 16 bits or (eight) 8."""
 
-    def __init__(self, rt, shapes, heads, kv_heads, pages, page_size=16, positions=8192, window=0):
+    def __init__(self, rt, shapes, heads, kv_heads, pages, page_size=16, positions=8192, window=0, eight=False):
         self.rt, self.heads, self.kv_heads, self.window = rt, heads, kv_heads, window
         self.size = {n: (rows, cols) for n, rows, cols in shapes}
         self.hidden, self.dim = self.size["q"][1], self.size["q"][0] // heads
-        self.cache = KvCache.empty(pages, kv_heads, page_size, self.dim)
+        self.cache = (KvCache8 if eight else KvCache).empty(pages, kv_heads, page_size, self.dim)
         turn = torch.arange(positions, dtype=torch.float64)[:, None] * 10000.0 ** (
             -torch.arange(0, self.dim, 2, dtype=torch.float64) / self.dim)
         self.cos, self.sin = turn.cos().float().cuda(), turn.sin().float().cuda()
@@ -73,32 +74,27 @@ class Sequences:
     KEPT = 8  # batches
 
     def __init__(self, layer, count, most):
-        page = layer.cache.k.shape[2]
+        pages, page = layer.cache.k.shape[0], layer.cache.k.shape[2]
         self.layer, self.page, self.most = layer, page, most
-        self.table = torch.full((count, -(-most // page)), -1, dtype=torch.int32, device="cuda")
-        self.kv_len = torch.zeros(count, dtype=torch.int32, device="cuda")
-        self.lengths, self.free = [0] * count, list(range(layer.cache.k.shape[0]))
-        self.pages = [[] for _ in range(count)]
+        self.pages = Pages.empty(pages, page, count, -(-most // page))
+        self.table, self.kv_len, self.lengths = self.pages.table, self.pages.kv_len, [0] * count
         self.steady = {}
 
-    def grow(self, news):
-        """Room for news[s] more tokens of every sequence, in the tensors that the batches read."""
-        for s, n in enumerate(news):
-            self.lengths[s] += n
-            while len(self.pages[s]) * self.page < self.lengths[s]:
-                self.table[s, len(self.pages[s])] = self.free[0]
-                self.pages[s].append(self.free.pop(0))
-        self.kv_len.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+    def grow(self, news, q_start=None):
+        """Room for news[s] more tokens of every sequence, in the tensors that the batches read; their rows' starts."""
+        self.lengths = [a + n for a, n in zip(self.lengths, news)]
+        if max(self.lengths) > self.most or sum(-(-n // self.page) for n in self.lengths) > self.pages.free.shape[0]:
+            raise RuntimeError("no pages left for %s tokens" % self.lengths)  # (known here without asking the GPU)
+        return self.pages.advance(torch.tensor(news, dtype=torch.int32, device="cuda"), rows=sum(news), q_start=q_start, places=False)[0]
 
     def batch(self, news):
         """The batch in which every sequence has news[s] new tokens; the last KEPT kinds of them are kept, each with its workspace
         (steps of single tokens and drafts come again and again, prompts hardly ever in the same lengths; who captures a call keeps
         its batch)."""
-        self.grow(news)
         key = tuple(news)
         batch = self.steady.pop(key, None)
+        starts = self.grow(news, batch and batch.tensors[0])
         if batch is None:
-            starts = torch.tensor([0] + news, dtype=torch.int32).cumsum(0, dtype=torch.int32).cuda()
             batch = Batch(self.layer.cache, self.layer.heads, starts, self.kv_len, self.table, max(news), self.most)
         self.steady[key] = batch  # (the last one used at the end)
         while len(self.steady) > self.KEPT:
@@ -109,6 +105,7 @@ class Sequences:
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     ap.add_argument("--small", action="store_true")
+    ap.add_argument("--cache8", action="store_true")
     ap.add_argument("--steps", type=int, default=32)
     a = ap.parse_args()
     shapes, heads, kv_heads = (SMALL, 8, 2) if a.small else (MISTRAL, 32, 8)
@@ -116,7 +113,7 @@ def main():
     with tempfile.TemporaryDirectory() as d:
         write_layer(d, shapes)
         with Runtime(d) as rt:
-            layer = Layer(rt, shapes, heads, kv_heads, pages=512)
+            layer = Layer(rt, shapes, heads, kv_heads, pages=512, eight=a.cache8)
             seqs = Sequences(layer, len(prompts), most=2000)
             torch.manual_seed(0)
 

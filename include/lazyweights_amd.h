@@ -319,8 +319,9 @@ int lw_attn8_prompt(const lw_kv8_cache* cache, const lw_batch* batch, int heads,
 
 /* The pages of `seqs` sequences (up to 8192) and the pool of those that none has, on the GPU: position j of sequence s
  * lies in row j % page_size of page table[s * table_stride + j / page_size]; free[0 .. left[0]) are the pool's pages, a
- * stack, of `pages` at most. page_size is a power of two up to 65536. workspace: 4 bytes, zero before its first use; calls leave
- * it zero, and calls that share one must not overlap. */
+ * stack, of `pages` at most. page_size is a power of two up to 65536. workspace: LW_PAGES_WORKSPACE bytes, zero before its first use;
+ * calls leave it zero, and calls that share one must not overlap. */
+enum { LW_PAGES_WORKSPACE = 1088 };
 typedef struct lw_pages {
   int32_t* table;
   int64_t table_stride;
@@ -338,7 +339,7 @@ typedef struct lw_pages {
  * sums of new_tokens before each sequence, the rows of a call (lw_batch); position[t], slot[t]: the position of row t and
  * page * page_size + its row there, -1 where the page is outside [0, pages) (either may be NULL). left_out[0]: pages left; left_out[1]:
  * 0, or what the call would have lacked, the sum of 1: pages, 2: room in the table, 4: rows. Then nothing is changed:
- * the lengths and the pool are what they were, q_start is all 0. kv_len_out and left_out may be the pages' own. Table entries
+ * the lengths and the pool are what they were, q_start is all 0. kv_len_out and left_out may be the pages' own (no other output may lie over an input). Table entries
  * past a sequence's pages, and rows past the last, are left as they were. Negative numbers count as 0. Asynchronous on
  * `stream`, allocates nothing, can be captured. Returns 0 or -1. */
 int lw_pages_advance(const lw_pages* pages, const int32_t* new_tokens, const int32_t* keep, int rows, int32_t* kv_len_out,

@@ -116,6 +116,7 @@ struct PagesArgs {
   int32_t *kv_len_out, *left_out, *q_start, *position, *count;
   int64_t *slot, tstride;
   int seqs, table_pages, pages, page_shift, rows;
+  bool in_place;  // an output is an input
 };
 
 hipError_t launch_append(const AppendArgs& a, int head_dim, int type, int x_type, hipStream_t s);

@@ -8,8 +8,10 @@ namespace lw {
 
 namespace {
 
+constexpr int H = 2, KEYS = 16 * H;  // of a tile: blocks of 16 keys that share an exponent, keys
+
 // LDS of a wave: its V tile and the weights of 32 keys, then [D][16] sums
-constexpr int decode8_wave(int dim, int blocks) { return std::max(16 * blocks * dim + 32 * 16 * 4, 64 * dim); }
+constexpr int decode8_wave(int dim) { return std::max(KEYS * dim + 32 * 16 * 4, 64 * dim); }
 
 // The part of an item that a block has. Items are (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as
 // many tiles of KEYS keys as the sequence's rows see together. A part takes `run` tiles at most, the tiles of all items / spare, so that
@@ -22,7 +24,7 @@ struct Part {
   int s, kvh, rb, lo, t_from, t_to;
   int base_slot, part, active;
 };
-template <int NW, int KEYS>
+template <int NW>
 __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles_l, uint32_t* parts_l, int lane, int w, Part& p) {
   const AttnArgs& a = args.a;
   const KvView& c = a.c;
@@ -130,12 +132,12 @@ __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles
   return true;
 }
 
-template <int D, bool BF, int RT, int NW, int H>
+template <int D, bool BF, int RT, int NW>
 __device__ __forceinline__ void decode8_part(const Attn8Args& args, uint8_t* smem, float* ml, int* last_block, const Part& p0, int lane,
                                              int w, int n, int g) {
-  constexpr int KEYS = 16 * H, C = D / 32, DT = D / 16, NP = 2, FULL = D / 64, TAIL = C % 2;
+  constexpr int C = D / 32, DT = D / 16, NP = 2, FULL = D / 64, TAIL = C % 2;
   constexpr float LIFT = lift<false>(0);
-  constexpr int WAVE = decode8_wave(D, H);
+  constexpr int WAVE = decode8_wave(D);
   const AttnArgs& a = args.a;
   const KvView& c = a.c;
   const Seq& sq = p0.sq;
@@ -362,38 +364,38 @@ __device__ __forceinline__ void decode8_part(const Attn8Args& args, uint8_t* sme
 // counted 2; the last part's join 2 to 4 more.
 //
 // RUNS: a block has an equal run of the list of all items' tiles (walk_items) instead of a part.
-template <int D, bool BF, int RT, int NW, int H, bool RUNS>
+template <int D, bool BF, int RT, int NW, bool RUNS>
 __global__ __launch_bounds__(64 * NW, RT == 1 && !RUNS ? 4 : 2) void k_attn8_decode(const Attn8Args args) {
   // the waves' V tiles, and behind each the weights of 32 keys of the careful pass (after the loop their sums); then, of more than one
   // row tile, q
-  __shared__ __align__(16) uint8_t smem[NW * decode8_wave(D, H) + (RT > 1 ? NW * RT * 16 * D * 2 : 0)];
+  __shared__ __align__(16) uint8_t smem[NW * decode8_wave(D) + (RT > 1 ? NW * RT * 16 * D * 2 : 0)];
   __shared__ float ml[NW * 16 * RT * 2];
   __shared__ uint32_t csum[RUNS ? 1024 : 1];
   __shared__ int last_block;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   if constexpr (RUNS) {
-    walk_items<NW, 16 * H>(args.a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0,
+    walk_items<NW, KEYS>(args.a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0,
                                                       int T, uint32_t run) __attribute__((always_inline)) {
       // (a block's number is that of its run in the list)
       const int b0 = (int)(item0 / run), b1 = (int)((item0 + T - 1) / run);
       const Part p = {sq, s, kvh, rb, lo, t_from, t_to, b0, (int)blockIdx.x - b0, b1 - b0 + 1};
-      decode8_part<D, BF, RT, NW, H>(args, smem, ml, &last_block, p, lane, w, n, g);
+      decode8_part<D, BF, RT, NW>(args, smem, ml, &last_block, p, lane, w, n, g);
     });
   } else {
     Part p;
     uint32_t* sums_l = reinterpret_cast<uint32_t*>(smem);  // of tiles and of parts of the sequences up to each 64th
-    if (find_part<NW, 16 * H>(args, sums_l, sums_l + 1024, lane, w, p))
-      decode8_part<D, BF, RT, NW, H>(args, smem, ml, &last_block, p, lane, w, n, g);
+    if (find_part<NW>(args, sums_l, sums_l + 1024, lane, w, p))
+      decode8_part<D, BF, RT, NW>(args, smem, ml, &last_block, p, lane, w, n, g);
   }
 }
 
 template <int D, bool BF>
 hipError_t decode8_d(const Attn8Args& a, const DecodePlan& p, hipStream_t s) {
   const dim3 grid((uint32_t)p.blocks);
-  if (p.row_tiles == 2) k_attn8_decode<D, BF, 2, 4, 2, false><<<grid, 256, 0, s>>>(a);
-  else if (D == 128 && p.runs) k_attn8_decode<128, BF, 1, 4, 2, true><<<grid, 256, 0, s>>>(a);
-  else if (p.waves == 8) k_attn8_decode<D, BF, 1, 8, 2, false><<<grid, 512, 0, s>>>(a);
-  else k_attn8_decode<D, BF, 1, 4, 2, false><<<grid, 256, 0, s>>>(a);
+  if (p.row_tiles == 2) k_attn8_decode<D, BF, 2, 4, false><<<grid, 256, 0, s>>>(a);
+  else if (D == 128 && p.runs) k_attn8_decode<128, BF, 1, 4, true><<<grid, 256, 0, s>>>(a);
+  else if (p.waves == 8) k_attn8_decode<D, BF, 1, 8, false><<<grid, 512, 0, s>>>(a);
+  else k_attn8_decode<D, BF, 1, 4, false><<<grid, 256, 0, s>>>(a);
   return hipGetLastError();
 }
 

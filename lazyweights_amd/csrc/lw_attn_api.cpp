@@ -327,6 +327,7 @@ int lw_pages_advance(const lw_pages* p, const int32_t* new_tokens, const int32_t
   if (p->pages < 0 || p->pages >= kMostRows || rows < 0 || rows >= kMostRows) return refuse(fn, "pages or rows out of range");
   if (p->table_pages < 0 || p->table_stride < p->table_pages || (long long)p->table_pages * p->page_size >= kMostRows)
     return refuse(fn, "the table holds 2^30 positions or more, or its stride is less than its pages");
+  if (reinterpret_cast<uintptr_t>(p->workspace) & 3) return refuse(fn, "workspace not aligned to 4");
   if (!q_start || !left_out || !p->left || !p->workspace || (p->pages > 0 && !p->free)) return refuse(fn, "null array");
   if (p->seqs > 0 && (!p->kv_len || !kv_len_out || !new_tokens || (p->table_pages > 0 && !p->table))) return refuse(fn, "null array");
   lw::PagesArgs a;
@@ -348,6 +349,7 @@ int lw_pages_advance(const lw_pages* p, const int32_t* new_tokens, const int32_t
   a.pages = p->pages;
   a.page_shift = __builtin_ctz((unsigned)p->page_size);
   a.rows = rows;
+  a.in_place = left_out == p->left || kv_len_out == p->kv_len || kv_len_out == new_tokens || kv_len_out == keep;
   return launched(fn, lw::launch_pages(a, static_cast<hipStream_t>(stream)));
 }
 

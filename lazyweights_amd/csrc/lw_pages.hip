@@ -9,7 +9,7 @@ namespace lw {
 namespace {
 
 constexpr int kMost = 1 << 30;  // sums are counted up to here, so that they fit 32 bits whatever the arrays hold
-constexpr int kPageThreads = 512;
+constexpr int kPageThreads = 512, kGroups = 16;
 
 __device__ __forceinline__ int add_up(int x, int y) { return min(x + y, kMost); }
 
@@ -27,7 +27,12 @@ __device__ __forceinline__ int find(const int* first, int n, int x) {
 // Every block adds up all sequences' new rows, pages taken and pages given (sums before each in LDS), so that one launch needs
 // no exchange between blocks; then the blocks share the rows and the pages that change hands, each found by
 // bisection. What the step reads (table entries up to the old lengths, the pool up to its count) it does not write (entries
-// and places behind these): only lengths and count may be given in place, and the block that has read them last writes those.
+// and places behind these): only lengths and count may be given in place, and then the block that has read them last writes those. It
+// is found by counters in two levels, since additions to one take 65 ns each, one after the other (500 sequences with 216000 rows in
+// 422 blocks; kGroups counters on lines of their own).
+//
+// Bound by latency: the arrays, the sums, a bisection, a page: a few thousand cycles in turn, over as many threads as there are rows
+// (a row per thread: 500 sequences, 216000 rows 7.5 us, four rows 13; 64 sequences 4.5).
 template <int SEQS>
 __global__ __launch_bounds__(kPageThreads) void k_pages(const PagesArgs a) {
   constexpr int T = kPageThreads, PER = (SEQS + T - 1) / T, WAVES = T / 64;
@@ -99,9 +104,15 @@ __global__ __launch_bounds__(kPageThreads) void k_pages(const PagesArgs a) {
   __syncthreads();
   // this block is done with what may be overwritten
   if (t == 0) {
-    const uint32_t n = gridDim.x == 1 ? 0 : __hip_atomic_fetch_add(reinterpret_cast<uint32_t*>(a.count), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    last = n == gridDim.x - 1;
-    if (last && n) __hip_atomic_store(a.count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    auto arrive = [&](int counter, uint32_t of) {  // whether this is the last of so many; the counter is 0 again then
+      int32_t* count = a.count + 16 * counter;
+      const bool end = (uint32_t)__hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1;
+      if (end) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return end;
+    };
+    const uint32_t group = blockIdx.x % kGroups;
+    if (gridDim.x == 1 || !a.in_place) last = blockIdx.x == 0;
+    else last = arrive(1 + group, (gridDim.x - group + kGroups - 1) / kGroups) && arrive(0, min(gridDim.x, (uint32_t)kGroups));
   }
   __syncthreads();
   if (last) {
@@ -148,7 +159,8 @@ __global__ __launch_bounds__(kPageThreads) void k_pages(const PagesArgs a) {
 }  // namespace
 
 hipError_t launch_pages(const PagesArgs& a, hipStream_t s) {
-  const int blocks = std::max(1, std::min(256, (a.rows + 4 * kPageThreads - 1) / (4 * kPageThreads)));
+  // (as many as are on the card at once: of 8192 sequences, with 128 KB of LDS, one per CU)
+  const int blocks = std::max(1, std::min(a.seqs <= kPageThreads ? 1024 : 256, (a.rows + kPageThreads - 1) / kPageThreads));
   if (a.seqs <= kPageThreads) k_pages<kPageThreads><<<blocks, kPageThreads, 0, s>>>(a);
   else k_pages<kMostPageSeqs><<<blocks, kPageThreads, 0, s>>>(a);
   return hipGetLastError();

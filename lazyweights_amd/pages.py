@@ -44,7 +44,7 @@ class Pages:
             raise ValueError("up to 8192 sequences")
         self.lib, self.index, self.seqs = load_library(), kv_len.get_device(), seqs
         self.page_size, self.kv_len, self.table, self.free, self.left = page_size, kv_len, table, free, left
-        self.workspace = torch.zeros(1, dtype=torch.int32, device=kv_len.device)
+        self.workspace = torch.zeros(272, dtype=torch.int32, device=kv_len.device)
         self._current, self._device = _current_stream(), _current_device()
         self.c = _Pages(table.data_ptr(), table.stride(0) if seqs > 1 else table.shape[1], table.shape[1], seqs, page_size,
                         free.shape[0], free.data_ptr(), kv_len.data_ptr(), left.data_ptr(), self.workspace.data_ptr())
