@@ -18,10 +18,11 @@ hipError_t prompt8_w(const Attn8Args& args, int splits, hipStream_t s) {
 template <int D, bool BF>
 hipError_t prompt8_d(const Attn8Args& args, hipStream_t s) {
   const AttnArgs& a = args.a;
-  // 8 waves where there is such a block for every CU: a tile is converted for twice as many rows (us with 8 / 4: 712 blocks of ragged
-  // prompts, 32 heads of 96, fp32 out 140 / 149, 500 of 4000 tokens, fp32 out 214 / 248, 1000 of 4 x 2000, heads of 64 140 / 150)
+  // 8 waves where there is such a block for most of the CUs: a tile is converted for twice as many rows (us with 8 / 4 waves: 712 blocks
+  // of ragged prompts, 32 heads of 96, fp32 out 135 / 149; 500 of 4000 tokens, fp32 out 198 / 248; 187 of 1500 tokens 51 / 56; 175
+  // of 1400 after 3000 129 / 140; 225 of 1800, fp32 out 77 / 73)
   const int64_t blocks = (int64_t)a.c.tokens * a.group / 256 * a.c.kv_heads;
-  if (blocks >= 256) return prompt8_w<D, BF, 8>(args, 1, s);
+  if (blocks >= 160) return prompt8_w<D, BF, 8>(args, 1, s);
   hipError_t e = prompt8_w<D, BF, 4>(args, a.splits, s);
   if (e == hipSuccess && a.splits > 1) {
     k_attn_join<D><<<dim3((uint32_t)prompt_items(a.c.seqs, a.c.kv_heads, a.group, a.c.tokens) * (D / 32)), 256, 0, s>>>(a);

@@ -146,6 +146,17 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
     const int ch = 2 * (lane >> 3) + i, row = 8 * (w & 1) + (lane & 7);
     put_at[i] = 2 * ((w >> 1) * BLK + ch * 128 + ((row + 4 * ch) & 15) * 8);
   }
+  // Of 8 waves, those of even units see to K's exponents and those of odd ones, the other halves of the same blocks, to V's; of 4 each
+  // sees to both, since a branch costs more there (15999 tokens 2074 us against 2173, but 2000 tokens 77 / 68).
+  constexpr bool PARITY = W == 8;
+  const uint8_t* kb8 = reinterpret_cast<const uint8_t*>(c.k) + kvh * c.hstride;
+  const uint8_t* vb8 = reinterpret_cast<const uint8_t*>(c.v) + kvh * c.hstride;
+  const int8_t *ke8 = nullptr, *ve8 = nullptr;
+  if constexpr (F8) {
+    ve8 = args.e.v + kvh * args.e.hstride;
+    ke8 = PARITY && w & 1 ? ve8 : args.e.k + kvh * args.e.hstride;
+  }
+  const uint32_t lane_off = (uint32_t)(lane & 7) * (uint32_t)c.rstride + 16 * min(lane >> 3, D / 16 - 1);
   u32x4 raw[F8 ? PIECES : 1];
   int raw_e[F8 ? PIECES : 1];
   uint32_t raw_pg[UNITS];
@@ -163,13 +174,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
       const int key = unit_key(t, u), in_page = key & ((1 << c.page_shift) - 1);
       raw_there[u] = page < c.pages;
       const int64_t at = raw_there[u] ? page : 0;
-      const int64_t off = at * c.pstride + kvh * c.hstride + (int64_t)in_page * c.rstride;
-      const int64_t eoff = at * args.e.pstride + kvh * args.e.hstride + in_page / kExpBlock;
-      const uint32_t mine = (uint32_t)min(lane & 7, hi - 1 - key) * (uint32_t)c.rstride + 16 * min(lane >> 3, D / 16 - 1);
-      raw[2 * u] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(c.k) + off + mine);
-      raw[2 * u + 1] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint8_t*>(c.v) + off + mine);
-      raw_e[2 * u] = args.e.k[eoff];
-      raw_e[2 * u + 1] = args.e.v[eoff];
+      const int64_t off = at * c.pstride + (int64_t)((uint64_t)(uint32_t)in_page * (uint32_t)c.rstride);
+      const int64_t eoff = at * args.e.pstride + in_page / kExpBlock;
+      uint32_t mine = lane_off;
+      if (W == 4 || hi - key < 8) mine = (uint32_t)min(lane & 7, hi - 1 - key) * (uint32_t)c.rstride + 16 * min(lane >> 3, D / 16 - 1);
+      raw[2 * u] = *reinterpret_cast<const u32x4*>(kb8 + off + mine);
+      raw[2 * u + 1] = *reinterpret_cast<const u32x4*>(vb8 + off + mine);
+      raw_e[2 * u] = ke8[eoff];
+      if (!PARITY) raw_e[2 * u + 1] = ve8[eoff];
     }
   };
   auto load = [&](int t) {
@@ -195,9 +207,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_prompt(const ARGS args) {
         for (int i = 0; i < 2; ++i)
           *reinterpret_cast<u32x4*>(reinterpret_cast<uint8_t*>(to) + put_at[i]) =
               j & 1 ? widen8<false>(raw[j][2 * i], raw[j][2 * i + 1]) : widen8<BF>(raw[j][2 * i], raw[j][2 * i + 1]);
-      // (the same values from every lane, and from the two units of a block)
-      const int to_tile = (t + 1) & 1, e = clampi(raw_e[j], -kMostExp, kMostExp);
-      if (j & 1) {
+      if (PARITY && j & 1) return;
+      const int to_tile = (t + 1) & 1;
+      const int e = clampi(PARITY ? __builtin_amdgcn_readfirstlane(raw_e[j]) : raw_e[j], -kMostExp, kMostExp);
+      if (PARITY ? w & 1 : j & 1) {  // (the same values from every lane; of 4 waves from the two units of a block)
         ve_l[to_tile][block] = (float)e;
         iv_l[to_tile][block] = two_to(-e);
       } else {
