@@ -135,10 +135,6 @@ class KvCache:
     def _memory(self):
         return self.k, self.v
 
-    def _q_dtype(self, q_out):
-        """The type that q gets when it is appended, into q_out if that is given."""
-        return self.k.dtype
-
     def _rows(self, what, x, heads):
         """Address and row stride of x [tokens, heads, head_dim] or [tokens, heads * head_dim]."""
         shape, stride, dim = x.shape, x.stride(), self.head_dim
@@ -188,9 +184,10 @@ class KvCache:
         kp, ldk = self._rows("k", k, self.kv_heads)
         vp, ldv = self._rows("v", v, self.kv_heads)
         other = None if stream is None else self._other(stream)
-        qp, ldq, op, ldo, q_dtype = None, 0, None, 0, self._q_dtype(q_out)
+        qp, ldq, op, ldo, q_dtype = None, 0, None, 0, None
         if q is not None:
             qp, ldq = self._rows("q", q, heads)
+            q_dtype = self._q_dtype(q_out) if self.eight else self.k.dtype
             if q_out is None:
                 q_out = self._empty((n, heads, self.head_dim), q_dtype, other)
             elif q_out.dtype != q_dtype or q_out.shape[0] != n:
@@ -204,12 +201,13 @@ class KvCache:
                 raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
             cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), min(cos.shape[0], (1 << 31) - 1), 2 * cos.shape[1]
         batch.c.tokens = n
-        args = (self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows, 1 if neighbours else 0, op)
         where = self._current(self.index) if stream is None else stream
         if self.eight:
-            rc = self.lib.lw_kv8_append(*args, self.types[q_dtype], ldo, where)
+            rc = self.lib.lw_kv8_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
+                                        1 if neighbours else 0, op, F16 if q is None else self.types[q_dtype], ldo, where)
         else:
-            rc = self.lib.lw_kv_append(*args, ldo, where)
+            rc = self.lib.lw_kv_append(self.ptr, batch.ptr, heads, qp, kp, vp, kind, ldq, ldk, ldv, cp, sp, rot, rows,
+                                       1 if neighbours else 0, op, ldo, where)
         if rc != 0:
             raise RuntimeError(last_error())
         if other is not None:
@@ -229,7 +227,7 @@ class KvCache:
             raise ValueError("the batch is for caches in %d bits" % (8 if batch.eight else 16))
         if not 0 <= window < 1 << 31:  # (32 bits in the call: no position is that far back)
             window = (1 << 31) - 1 if window > 0 else -1
-        if q.dtype != self._q_dtype(q):
+        if q.dtype != (self._q_type(q.dtype) if self.eight else self.k.dtype):
             raise ValueError("q must have the cache's type")
         qp, ldq = self._rows("q", q, heads)
         other = None if stream is None else self._other(stream)
@@ -240,12 +238,11 @@ class KvCache:
             raise ValueError("out must be float32, float16 or bfloat16, with q's rows")
         op, ldo = self._rows("out", out, heads)
         batch.c.tokens = q.shape[0]
-        args = (op, kind, ldo, self.head_dim ** -0.5 if scale is None else scale, window,
-                self._current(self.index) if stream is None else stream)
+        scale, where = self.head_dim ** -0.5 if scale is None else scale, self._current(self.index) if stream is None else stream
         if self.eight:
-            rc = call(self.ptr, batch.ptr, heads, qp, self.types[q.dtype], ldq, *args)
+            rc = call(self.ptr, batch.ptr, heads, qp, self.types[q.dtype], ldq, op, kind, ldo, scale, window, where)
         else:
-            rc = call(self.ptr, batch.ptr, heads, qp, ldq, *args)
+            rc = call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, scale, window, where)
         if rc != 0:
             raise RuntimeError(last_error())
         if other is not None:
@@ -314,6 +311,7 @@ class KvCache8(KvCache):
         return dtype
 
     def _q_dtype(self, q_out):
+        """The type that q gets when it is appended, into q_out if that is given."""
         return self.q_dtype if q_out is None else self._q_type(q_out.dtype)
 
     def attend_decode(self, batch, q, out=None, scale=None, window=0, stream=None):

@@ -382,7 +382,7 @@ __global__ __launch_bounds__(64 * NW, RT == 1 && !RUNS ? 4 : 2) void k_attn8_dec
       decode8_part<D, BF, RT, NW>(args, smem, ml, &last_block, p, lane, w, n, g);
     });
   } else {
-    Part p;
+    Part p = {};
     uint32_t* sums_l = reinterpret_cast<uint32_t*>(smem);  // of tiles and of parts of the sequences up to each 64th
     if (find_part<NW>(args, sums_l, sums_l + 1024, lane, w, p))
       decode8_part<D, BF, RT, NW>(args, smem, ml, &last_block, p, lane, w, n, g);
@@ -421,11 +421,12 @@ DecodePlan decode8_plan(int seqs, int kv_heads, int group, int head_dim, int max
   p.blocks_log2 = 9;
   // Parts: few items in about as many blocks as there are CUs (the more parts of an item, the longer its join: one of 131071 keys with
   // 248 spare blocks 58 us, 504 60, 1016 82; one of 30000 19, 25, 41), some more for items that are shorter (128 of 1000-3000 keys with
-  // 248 24, 504 20); many items so that a part is of some 100 tiles at the bounds.
+  // 248 24, 504 20); many items so that a part is of some 100 tiles at the bounds (512 of two row tiles, 500-16000 keys, with 1024
+  // 183, 2048 194).
   const int64_t few = items <= 64 ? 256 - items : std::max<int64_t>(512 - items, 256);
-  const int64_t many = std::min<int64_t>(std::max<int64_t>(tiles / 96, 512), 2048);
+  const int64_t many = std::min<int64_t>(std::max<int64_t>(tiles / 96, 512), p.row_tiles == 2 ? 1024 : 2048);
   p.spare = (int)std::max<int64_t>(1, std::min<int64_t>(items > 256 ? many : few, (tiles + 3) / 4));
-  p.blocks = p.runs ? 1 << p.blocks_log2 : (int)items + (p.whole ? 0 : p.spare);
+  p.blocks = p.runs ? 1 << p.blocks_log2 : (int)std::min<int64_t>(items + (p.whole ? 0 : p.spare), 1 << 30);
   // 8 waves where one block of a CU has a long part: half as many parts would leave half of the CUs idle, and 4 waves ask for too little
   // at a time (one of 131071 keys 55 / 58; one of 778 10.4 / 8.2)
   p.waves = !p.whole && items <= 64 && tiles / p.spare >= 64 ? 8 : 4;

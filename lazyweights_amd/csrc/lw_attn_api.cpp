@@ -213,6 +213,7 @@ int attend8(const char* fn, bool decode, const lw_kv8_cache* cache, const lw_bat
   if (decode && batch->max_new > 16) return refuse(fn, "max_new is more than 16 (lw_attn8_prompt takes any number)");
   if (decode) {
     const lw::DecodePlan p = lw::decode8_plan(batch->seqs, cache->kv_heads, a.a.group, cache->head_dim, batch->max_new, batch->max_kv);
+    if (p.blocks > kMostBlocks) return refuse(fn, "more sequences and heads than a launch can take");
     if (!take_plan(fn, p, batch, a.a)) return -1;
     return launched(fn, lw::launch_attn8_decode(a, p, cache->head_dim, q_type, static_cast<hipStream_t>(stream)));
   }

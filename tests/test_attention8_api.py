@@ -73,6 +73,13 @@ def test_decode_limits_and_workspace(lib):
         assert attend(lib, "decode", c, b) == -1 and attend(lib, "prompt", c, b) == -1 and append(lib, c, b) == -1
 
 
+def test_more_items_than_a_launch_takes(lib):
+    from lazyweights_amd import last_error
+    c = cache(kv_heads=1024, head_stride=0)
+    b = batch(seqs=65535, tokens=1024, max_kv=16, workspace_bytes=1 << 50)
+    assert attend(lib, "decode", c, b, heads=1024, ldq=1024 * 128, ldo=1024 * 128) == -1 and "more sequences" in last_error()
+
+
 def test_nothing_to_do(lib):
     for b in (batch(seqs=0), batch(tokens=0)):
         assert attend(lib, "decode", cache(), b) == 0 and attend(lib, "prompt", cache(), b, q_type=BF16) == 0

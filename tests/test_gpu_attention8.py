@@ -722,3 +722,64 @@ def test_python_refusals(gpu, lib):
         with pytest.raises(ValueError, match="bits"):
             call()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("call", ("attend_decode", "attend_prompt"))
+def test_rows_of_no_sequence_and_before_the_first_position(gpu, lib, call):
+    """Rows behind the last sequence's are left as they were; of a sequence with more rows than its length the first ones are before
+    its first position: nothing is appended for them, and they see nothing."""
+    import torch
+    m = Made(torch, (8, 2, 128), 16, "float16", [(3, 40), (5, 30)], 33)
+    m.kv_len[1] = 2  # of the second's 5 rows, 3 come before position 0
+    m.lengths = [(3, 40), (2, 0)]
+    before = [t.view(torch.uint8).clone() for t in (m.k, m.v, m.k_exp, m.v_exp)]
+    g = torch.Generator(device="cuda").manual_seed(34)
+    x = torch.randn((11, 2, 128), generator=g, device="cuda")
+    q = torch.randn((11, 8, 128), generator=g, device="cuda")
+    q16 = m.cache.append(m.batch, q, x, 2 * x, q_out=torch.full((11, 8, 128), float("nan"), dtype=torch.float16, device="cuda"))
+    real = torch.tensor([0, 1, 2, 6, 7], device="cuda")
+    assert torch.equal(q16[real], q[real].half()) and torch.isnan(q16[3:6]).all() and torch.isnan(q16[8:]).all()
+    first = int(m.table[1, 0])
+    for now, was in zip((m.k, m.v), before):
+        assert torch.equal(now.view(torch.uint8)[first, :, 2:], was[first, :, 2:])
+    e = m.k_exp[first, :, 0].double()
+    got = m.k.view(torch.uint8)[first, :, :2].view(torch.float8_e4m3fn).double() * torch.exp2(e)[:, None, None]
+    want = x[6:8].transpose(0, 1).double()
+    assert ((got - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** -10 * torch.exp2(e)[:, None, None]).all()
+    q16[torch.isnan(q16)] = 1
+    m.q = q16[real]
+    ref = reference(m)
+    y = getattr(m.cache, call)(m.batch, q16, out=torch.full((11, 8, 128), float("nan"), device="cuda"))
+    check(torch, y[real], ref, call == "attend_prompt")
+    assert not y[3:6].any() and torch.isnan(y[8:]).all()
+
+
+def test_two_batches_at_once(gpu, lib):
+    """Calls of two batches over one cache that overlap on two streams, eager and as captured graphs, give each its own result."""
+    import torch
+    from lazyweights_amd import Batch
+    m = Made(torch, (8, 2, 128), 16, "float16", [(1, 3000), (2, 4100), (1, 60)], 35)
+    other = Batch(m.cache, 8, m.q_start, m.kv_len, m.table, m.max_new, m.max_kv)
+    want = m.cache.attend_decode(m.batch, m.q, out=m.empty(torch.float32)).clone()
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], [torch.empty_like(want) for _ in range(2)]
+    torch.cuda.synchronize()
+    for batch, out in zip((m.batch, other), outs):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                m.cache.attend_decode(batch, m.q, out=out)
+        graphs.append(graph)
+    for step in range(4):
+        for out in outs:
+            out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for side, graph, batch, out in zip(sides, graphs, (m.batch, other), outs):
+            with torch.cuda.stream(side):
+                if step % 2:
+                    graph.replay()
+                else:
+                    for _ in range(20):
+                        m.cache.attend_decode(batch, m.q, out=out)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want), step
