@@ -284,8 +284,7 @@ int lw_attn_prompt(const lw_kv_cache* cache, const lw_batch* batch, int heads, c
  * no infinities); each block of 16 rows of a head has an exponent e in k_exp (v_exp)[p * exp_page_stride + h *
  * exp_head_stride + r / 16], -48 to 48 (others are taken as the nearer of these): an element is its number times 2^e.
  * Pages of page_size rows, a power of two from 16 to 65536; byte strides are multiples of 16 (row_stride less than 2^26), k and
- * v aligned to 16 bytes. Calls
- * are made with the cache's GPU as the calling thread's current one, where `stream` is. */
+ * v aligned to 16 bytes. Calls are made with the cache's GPU as the calling thread's current one, where `stream` is. */
 typedef struct lw_kv8_cache {
   void* k;
   void* v;

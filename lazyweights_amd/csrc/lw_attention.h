@@ -1,6 +1,6 @@
 // Attention over a paged key-value cache: arguments of the kernels and their launchers (host interface of
-// lw_attn_decode.hip and lw_attn_prompt.hip, of lw_attn8.hip over a cache in 8 bits and of lw_pages.hip; the C-ABI in
-// lw_attn_api.cpp checks what a caller gives and fills these).
+// lw_attn_decode.hip and lw_attn_prompt.hip, of lw_kv8_append.hip, lw_attn8_decode.hip and lw_attn8_prompt.hip over a cache in
+// 8 bits and of lw_pages.hip; the C-ABI in lw_attn_api.cpp checks what a caller gives and fills these).
 #pragma once
 #include <hip/hip_runtime.h>
 

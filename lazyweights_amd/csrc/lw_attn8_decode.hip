@@ -28,7 +28,7 @@ template <int NW>
 __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles_l, uint32_t* parts_l, int lane, int w, Part& p) {
   const AttnArgs& a = args.a;
   const KvView& c = a.c;
-  const int seqs = c.seqs, kv_heads = c.kv_heads, H = kv_heads * a.row_blocks, chunks = (seqs + 63) >> 6;
+  const int seqs = c.seqs, kv_heads = c.kv_heads, of_seq = kv_heads * a.row_blocks, chunks = (seqs + 63) >> 6;
   // tiles of each of a sequence's items: those of the keys [lo, len) that its rows see; one where they see none, to write
   // the zeros
   auto first_key = [&](const Seq& q) { return a.window > 0 ? max(0, q.len - q.rows - a.window + 1) & ~(KEYS - 1) : 0; };
@@ -36,8 +36,8 @@ __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles
   p.base_slot = p.part = 0;
   p.active = 1;
   if (a.whole) {
-    p.s = (int)blockIdx.x / H;
-    const int hb = (int)blockIdx.x - p.s * H;
+    p.s = (int)blockIdx.x / of_seq;
+    const int hb = (int)blockIdx.x - p.s * of_seq;
     p.rb = hb / kv_heads;
     p.kvh = hb - p.rb * kv_heads;
     p.sq = sequence(c, p.s);
@@ -69,9 +69,9 @@ __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles
   int chunk = 0;
   if (chunks == 1) {
     hold(0);
-    tiles = upto(T * H);
+    tiles = upto(T * of_seq);
     run = run_of(__builtin_amdgcn_readlane(tiles, min(seqs, 64) - 1));
-    parts = upto((T + run - 1) / run * H);
+    parts = upto((T + run - 1) / run * of_seq);
   } else {
     // sums up to each 64th sequence, of tiles and then, with the run that these give, of parts
     auto sums = [&](uint32_t* l, auto value) __attribute__((always_inline)) {
@@ -97,9 +97,9 @@ __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles
       }
       __syncthreads();
     };
-    sums(tiles_l, [&] { return T * H; });
+    sums(tiles_l, [&] { return T * of_seq; });
     run = run_of(__builtin_amdgcn_readfirstlane(tiles_l[chunks - 1]));
-    sums(parts_l, [&] { return (T + run - 1) / run * H; });
+    sums(parts_l, [&] { return (T + run - 1) / run * of_seq; });
     for (int i = 0; i < chunks; i += 64) chunk += __popcll(__ballot(i + lane < chunks && parts_l[min(i + lane, chunks - 1)] <= at));
     if (chunk && chunk < chunks) {
       tiles_before = __builtin_amdgcn_readfirstlane(tiles_l[chunk - 1]);
@@ -108,8 +108,8 @@ __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles
     __syncthreads();  // (the memory is used again)
     if (chunk >= chunks) return false;
     hold(chunk);
-    tiles = upto(T * H);
-    parts = upto((T + run - 1) / run * H);
+    tiles = upto(T * of_seq);
+    parts = upto((T + run - 1) / run * of_seq);
   }
   at -= parts_before;
   const int j = __ffsll((unsigned long long)__ballot(parts > at)) - 1;
@@ -118,8 +118,8 @@ __device__ __forceinline__ bool find_part(const Attn8Args& args, uint32_t* tiles
   p.sq = Seq{(int)of(mine.row0), (int)of(mine.rows), (int)of(mine.len)};
   p.s = 64 * chunk + j;
   const uint32_t t = of(T), each = (t + run - 1) / run;
-  at -= of(parts) - each * H;
-  tiles_before += of(tiles) - t * H;
+  at -= of(parts) - each * of_seq;
+  tiles_before += of(tiles) - t * of_seq;
   const uint32_t hb = at / each;
   p.rb = hb / kv_heads;
   p.kvh = hb - p.rb * kv_heads;

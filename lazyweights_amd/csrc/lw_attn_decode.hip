@@ -266,10 +266,7 @@ __device__ __forceinline__ void decode_item(const AttnArgs& a, uint8_t* smem, fl
   join_item<D, RT, NW>(a, smem, ml, last_block, m, l, o, s, sq, kvh, rb, b0, (int)blockIdx.x - b0, b1 - b0 + 1, w, n, g);
 }
 
-// Work is a list of items (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as many tiles of 32
-// keys as the sequence's rows see together; the launch's blocks take equal runs of the list's tiles, whatever the lengths.
-// Within a run, a block's waves take the tiles of an item in turn, each on its own (no barrier in the loop), and join at
-// the item's end. An item that lies in several runs is joined, in their order, by the block that ends last.
+// Work is divided by walk_items, in tiles of 32 keys.
 //
 // Each key and value is read once, for all rows of its key-value head: 2 x 2 x D bytes a key against 4 x D x rows operations, so
 // a few tens of rows are bound by memory and the matrix cores are used for their layout (an item of 4 rows fills a quarter of a

@@ -1,5 +1,5 @@
-// The division of decode attention's work over blocks (of a 16-bit cache) and the join of its parts (lw_attn_decode.hip,
-// lw_attn8_decode.hip).
+// The division of decode attention's work into equal runs of a list and the join of an item's parts (lw_attn_decode.hip, and
+// lw_attn8_decode.hip, which has parts of another division too).
 //
 // Work is a list of items (sequence, key-value head, block of RT tiles of 16 (token, head) rows), each as many tiles of KEYS
 // keys as the sequence's rows see together; the launch's blocks take equal runs of the list's tiles, whatever the lengths.
