@@ -136,7 +136,7 @@ class KvCache:
         return self.k, self.v
 
     def _rows(self, what, x, heads):
-        """Address and row stride of x [tokens, heads, head_dim] or [tokens, heads * head_dim]."""
+        """Rows, address and row stride of x [tokens, heads, head_dim] or [tokens, heads * head_dim]."""
         shape, stride, dim = x.shape, x.stride(), self.head_dim
         if len(shape) == 3:
             ok = shape[1] == heads and shape[2] == dim and stride[2] == 1 and (heads == 1 or stride[1] == dim)
@@ -145,7 +145,8 @@ class KvCache:
         if not ok or x.get_device() != self.index:
             raise ValueError("%s: [tokens, %d, %d] (or the two last joined) with contiguous rows on the cache's device is "
                              "wanted, not %s" % (what, heads, dim, tuple(shape)))
-        return x.data_ptr(), stride[0] if shape[0] > 1 else heads * dim
+        rows = shape[0]
+        return rows, x.data_ptr(), stride[0] if rows > 1 else heads * dim
 
     def _other(self, stream):
         """torch's stream of the handle `stream`; None if that is the current one."""
@@ -177,29 +178,31 @@ class KvCache:
                 return self.append(batch, q, k, v, cos, sin, q_out, neighbours, stream)
         if batch.index != self.index:
             raise ValueError("the batch is on another device than the cache")
-        heads, n = batch.heads, k.shape[0]
-        kind = self.types.get(k.dtype)
-        if kind is None or v.dtype != k.dtype or v.shape[0] != n or (q is not None and (q.dtype != k.dtype or q.shape[0] != n)):
+        heads, dtype = batch.heads, k.dtype
+        kind = self.types.get(dtype)
+        n, kp, ldk = self._rows("k", k, self.kv_heads)
+        nv, vp, ldv = self._rows("v", v, self.kv_heads)
+        nq, qp, ldq = (n, None, 0) if q is None else self._rows("q", q, heads)
+        if kind is None or v.dtype != dtype or nv != n or nq != n or (q is not None and q.dtype != dtype):
             raise ValueError("q, k and v must have one of the types float32, float16, bfloat16 and the same number of rows")
-        kp, ldk = self._rows("k", k, self.kv_heads)
-        vp, ldv = self._rows("v", v, self.kv_heads)
         other = None if stream is None else self._other(stream)
-        qp, ldq, op, ldo, q_dtype = None, 0, None, 0, None
+        op, ldo, q_dtype = None, 0, None
         if q is not None:
-            qp, ldq = self._rows("q", q, heads)
             q_dtype = self._q_dtype(q_out) if self.eight else self.k.dtype
             if q_out is None:
                 q_out = self._empty((n, heads, self.head_dim), q_dtype, other)
-            elif q_out.dtype != q_dtype or q_out.shape[0] != n:
+            no, op, ldo = self._rows("q_out", q_out, heads)
+            if q_out.dtype != q_dtype or no != n:
                 raise ValueError("q_out must have the cache's type and q's rows")
-            op, ldo = self._rows("q_out", q_out, heads)
         cp, sp, rot, rows = None, None, 0, 0
         if cos is not None or sin is not None:
-            if (cos is None or sin is None or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2
-                    or cos.shape != sin.shape or cos.get_device() != self.index or sin.get_device() != self.index
+            shape = () if cos is None else cos.shape
+            if (sin is None or len(shape) != 2 or cos.dtype != torch.float32 or sin.dtype != torch.float32
+                    or shape != sin.shape or cos.get_device() != self.index or sin.get_device() != self.index
                     or not cos.is_contiguous() or not sin.is_contiguous()):
                 raise ValueError("cos and sin must be contiguous float32 tensors [positions, rot / 2] on the cache's device")
-            cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), min(cos.shape[0], (1 << 31) - 1), 2 * cos.shape[1]
+            rows, rot = shape
+            cp, sp, rows, rot = cos.data_ptr(), sin.data_ptr(), min(rows, (1 << 31) - 1), 2 * rot
         batch.c.tokens = n
         where = self._current(self.index) if stream is None else stream
         if self.eight:
@@ -227,20 +230,21 @@ class KvCache:
             raise ValueError("the batch is for caches in %d bits" % (8 if batch.eight else 16))
         if not 0 <= window < 1 << 31:  # (32 bits in the call: no position is that far back)
             window = (1 << 31) - 1 if window > 0 else -1
-        if q.dtype != (self._q_type(q.dtype) if self.eight else self.k.dtype):
+        dtype = q.dtype
+        if dtype != (self._q_type(dtype) if self.eight else self.k.dtype):
             raise ValueError("q must have the cache's type")
-        qp, ldq = self._rows("q", q, heads)
+        n, qp, ldq = self._rows("q", q, heads)
         other = None if stream is None else self._other(stream)
         if out is None:
-            out = self._empty(q.shape, q.dtype, other)
+            out = self._empty(q.shape, dtype, other)
         kind = self.types.get(out.dtype)
-        if kind is None or out.shape[0] != q.shape[0]:
+        no, op, ldo = self._rows("out", out, heads)
+        if kind is None or no != n:
             raise ValueError("out must be float32, float16 or bfloat16, with q's rows")
-        op, ldo = self._rows("out", out, heads)
-        batch.c.tokens = q.shape[0]
+        batch.c.tokens = n
         scale, where = self.head_dim ** -0.5 if scale is None else scale, self._current(self.index) if stream is None else stream
         if self.eight:
-            rc = call(self.ptr, batch.ptr, heads, qp, self.types[q.dtype], ldq, op, kind, ldo, scale, window, where)
+            rc = call(self.ptr, batch.ptr, heads, qp, self.types[dtype], ldq, op, kind, ldo, scale, window, where)
         else:
             rc = call(self.ptr, batch.ptr, heads, qp, ldq, op, kind, ldo, scale, window, where)
         if rc != 0:

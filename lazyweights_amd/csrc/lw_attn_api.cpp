@@ -302,7 +302,7 @@ int lw_kv8_append(const lw_kv8_cache* cache, const lw_batch* batch, int heads, c
   const lw_kv_cache plain = shape(*cache);
   const int rc = append_args(fn, &plain, batch, heads, q, k, v, x_type, ldq, ldk, ldv, cos, sin, rot, rope_rows, neighbours, q_out, ldo, a.a);
   if (rc) return rc < 0 ? -1 : 0;
-  if (((long long)batch->tokens / lw::kExpBlock + 2ll * batch->seqs) * 2 * cache->kv_heads + (long long)batch->tokens * ((heads + 15) / 16) > kMostBlocks)
+  if (((long long)batch->tokens / lw::kExpBlock + 2ll * batch->seqs) * cache->kv_heads + (long long)batch->tokens * ((heads + 15) / 16) > kMostBlocks)
     return refuse(fn, "more tokens than a launch can take");
   a.e = exponents(*cache);
   return launched(fn, lw::launch_append8(a, cache->head_dim, q_type, x_type, static_cast<hipStream_t>(stream)));

@@ -118,13 +118,14 @@ __device__ __forceinline__ void add_exactly(float& sum, float& lost, float x) {
 struct Seq {
   int row0, rows, len;
 };
-__device__ __forceinline__ Seq sequence(const KvView& c, int s) {
+__device__ __forceinline__ Seq sequence(const KvView& c, int from, int to, int kv_len) {
   Seq q;
-  q.row0 = clampi(c.q_start[s], 0, c.tokens);
-  q.rows = clampi(c.q_start[s + 1], q.row0, c.tokens) - q.row0;
-  q.len = clampi(c.kv_len[s], 0, c.table_pages << c.page_shift);  // (the host keeps that within 2^30)
+  q.row0 = clampi(from, 0, c.tokens);
+  q.rows = clampi(to, q.row0, c.tokens) - q.row0;
+  q.len = clampi(kv_len, 0, c.table_pages << c.page_shift);  // (the host keeps that within 2^30)
   return q;
 }
+__device__ __forceinline__ Seq sequence(const KvView& c, int s) { return sequence(c, c.q_start[s], c.q_start[s + 1], c.kv_len[s]); }
 
 // element offset of key `key` of the sequence whose table row is `table`, and whether it is there
 __device__ __forceinline__ int64_t key_offset(const KvView& c, uint32_t page, int key, bool& there) {

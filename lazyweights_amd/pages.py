@@ -62,7 +62,7 @@ class Pages:
 
     def _whole(self, what, t, size, dtype=torch.int32):
         """Address of a contiguous tensor [size] of whole numbers on the pages' device."""
-        if t.dtype != dtype or t.shape != (size,) or t.get_device() != self.index or (size > 1 and t.stride(0) != 1):
+        if t.dtype != dtype or t.shape != (size,) or t.get_device() != self.index or not t.is_contiguous():
             raise ValueError("%s: %s [%d], contiguous, on the pages' device is wanted" % (what, dtype, size))
         return t.data_ptr()
 
