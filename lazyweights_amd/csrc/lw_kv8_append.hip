@@ -76,8 +76,7 @@ __global__ __launch_bounds__(2 * D) void k_kv8_append(const Append8Args args, ui
   };
   if (blockIdx.x >= kv_blocks) {
     const int parts = (a.heads + 15) / 16, b = blockIdx.x - kv_blocks, row = b / parts;
-    const int h = (b - row * parts) * 16 + threadIdx.x / U;
-    if (h >= a.heads) return;
+    const int head = (b - row * parts) * 16 + threadIdx.x / U, h = min(head, a.heads - 1);  // (all lanes search)
     const bool turn = 8 * unit < a.rot;
     int e0, e1;
     pieces(unit, turn, e0, e1);
@@ -86,7 +85,7 @@ __global__ __launch_bounds__(2 * D) void k_kv8_append(const Append8Args args, ui
     int s = min(row, c.seqs - 1);
     const Seq sq = find(s, row, [&](int, int from) { return from; });
     const int pos = sq.len - sq.rows + (row - sq.row0);
-    if (row < sq.row0 || row >= sq.row0 + sq.rows || pos < 0) return;
+    if (head >= a.heads || row < sq.row0 || row >= sq.row0 + sq.rows || pos < 0) return;
     if (turn) {
       angles(unit, pos, cs, sn);
       rotate(x, y, cs, sn, a.neighbours);

@@ -511,6 +511,9 @@ APPEND = [
     ((4, 2, 128), 16, "float16", "float32", 0, False, 1e-3, [(40, 1), (0, 0), (2, 2)]),
     ((20, 1, 128), 16, "float16", "float32", 128, False, 5, [(i % 3, 7 * i % 40) for i in range(200)]),
     ((1, 1, 64), 16, "float16", "float32", 64, False, 5, [(1, i) for i in range(90)]),
+    # (a wave with heads for some of its lanes only, and sequences to search)
+    ((3, 1, 64), 16, "float16", "float32", 64, False, 5, [(i % 3, 7 * i % 40) for i in range(200)]),
+    ((21, 7, 96), 16, "bfloat16", "float16", 96, True, 5, [(3 * i % 7, 5 * i % 90) for i in range(70)]),
 ]
 
 
