@@ -358,7 +358,7 @@ __device__ __forceinline__ void decode8_part(const Attn8Args& args, uint8_t* sme
 //
 // Bound by memory: 2 D + 1/8 bytes a key and key-value head. A wave has a tile of 32 keys (8 KB at D = 128) on its way while it works on the
 // one before; 128 registers leave room for 16 waves a CU (64 keys a tile and 8 waves: 64 sequences of 500-16000 keys 127 us against
-// 123, 256 of 100-2000 94 against 91). us, and of the bytes: 64 sequences of 500-16000 keys, 8 heads of 128: 123 (580 MB: 4.7
+// 123, 256 of 100-2000 94 against 91). us, and of the bytes: 64 sequences of 500-16000 keys, 8 heads of 128: 120 (580 MB: 4.8
 // TB/s); one of 131071: 55 (268 MB: 4.9, 5.4 in the loop); 4 x 5 tokens of 32 heads of 96 over 301-5003: 11.7 (50 MB); one of 778: 8.2.
 // A launch without its bytes is 6 us (200 keys: 6.7): start, lengths 1, page and first tile 1.5, stores of a part until they are
 // counted 2; the last part's join 2 to 4 more.
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(64 * NW, RT == 1 && !RUNS ? 4 : 2) void k_attn8_dec
   __shared__ int last_block;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
   if constexpr (RUNS) {
-    walk_items<NW, KEYS>(args.a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0,
+    walk_items<NW, KEYS, false>(args.a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0,
                                                       int T, uint32_t run) __attribute__((always_inline)) {
       // (a block's number is that of its run in the list)
       const int b0 = (int)(item0 / run), b1 = (int)((item0 + T - 1) / run);
@@ -413,19 +413,21 @@ DecodePlan decode8_plan(int seqs, int kv_heads, int group, int head_dim, int max
   // us), and where there are many, none long (us against parts: 1024 items of 300-1000 keys 42 / 44, 2048 of 100-2000 91 / 95; 512 of
   // two row tiles and 100-3000 keys 53 / 62; but 240 of 100-2000 20 / 18).
   p.whole = items <= 1 << 20 && (max_kv <= 256 || (p.row_tiles == 2 ? items >= 512 && max_kv <= 4096 : items >= 1024 && max_kv <= 2048));
-  // Equal runs of the list of all items, for 512 blocks, where there are many and long ones: what a CU has to read is then the same
+  // Equal runs of the list of all items, for 512 blocks, where there are many and not short ones: what a CU has to read is then the same
   // everywhere, and a CU takes little more than its share of the card's rate (parts end unevenly, whatever their number). us with runs
-  // / parts: 512 items of 500-16000 keys 123 / 133, 1024 of them 241 / 261, 512 of 8000 189 / 207, 2048 of 300-8000 248 / 283, 256 of
-  // 500-16000 66 / 71; 512 of 300-5000 58 / 61. Heads of 96, whose tiles are smaller, need more waves beside one another: 124 / 101.
-  p.runs = !p.whole && p.row_tiles == 1 && head_dim == 128 && items >= 256 && max_kv > 4096;
+  // / parts: 512 items of 500-16000 keys 144 / 148, of 8000 182 / 189, of 1500-3500 74 / 101, of 500-4000 62 / 75, 2048 of 1500-3500 235 /
+  // 306; 248 of 500-16000 67 / 84, 192 of 1500-3500 29 / 33; 128 of 20000-60000 207 / 228, of 8000 60 / 61, of 1500-3500 24 / 23; but
+  // 2048 of 100-2000 119 / 88. Heads of 96, whose tiles are smaller, need more waves beside one another: 512 of 500-16000 124 / 101.
+  p.runs = !p.whole && p.row_tiles == 1 && head_dim == 128 && (items > 128 ? max_kv > 2048 : items >= 64 && max_kv > 16384);
   p.blocks_log2 = 9;
   // Parts: few items in about as many blocks as there are CUs (the more parts of an item, the longer its join: one of 131071 keys with
   // 248 spare blocks 58 us, 504 60, 1016 82; one of 30000 19, 25, 41), some more for items that are shorter (128 of 1000-3000 keys with
   // 248 24, 504 20); many items so that a part is of some 100 tiles at the bounds (512 of two row tiles, 500-16000 keys, with 1024
-  // 183, 2048 194).
+  // 183, 2048 194; 248 items, us with many / few: heads of 64, 500-16000 keys 36 / 48, of 128, 300-1500 20 / 21; but 160 of heads
+  // of 96, 1500-3500 24 / 21, and 248 of two row tiles 71 / 59).
   const int64_t few = items <= 64 ? 256 - items : std::max<int64_t>(512 - items, 256);
   const int64_t many = std::min<int64_t>(std::max<int64_t>(tiles / 96, 512), p.row_tiles == 2 ? 1024 : 2048);
-  p.spare = (int)std::max<int64_t>(1, std::min<int64_t>(items > 256 ? many : few, (tiles + 3) / 4));
+  p.spare = (int)std::max<int64_t>(1, std::min<int64_t>(items > (p.row_tiles == 2 ? 256 : 192) ? many : few, (tiles + 3) / 4));
   p.blocks = p.runs ? 1 << p.blocks_log2 : (int)std::min<int64_t>(items + (p.whole ? 0 : p.spare), 1 << 30);
   // 8 waves where one block of a CU has a long part: half as many parts would leave half of the CUs idle, and 4 waves ask for too little
   // at a time (one of 131071 keys 55 / 58; one of 778 10.4 / 8.2)

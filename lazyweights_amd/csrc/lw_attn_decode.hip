@@ -285,7 +285,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_decode(const AttnArgs a) {
   __shared__ uint32_t csum[1024];  // tiles of the sequences up to each 64th
   __shared__ int last_block;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
-  walk_items<NW, 32>(a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0, int T,
+  walk_items<NW, 32, true>(a, csum, lane, w, [&](int s, const Seq& sq, int kvh, int rb, int lo, int t_from, int t_to, uint32_t item0, int T,
                                            uint32_t run) __attribute__((always_inline)) {
     decode_item<D, BF, RT, NW>(a, smem, ml, pcare, &last_block, s, sq, kvh, rb, lo, t_from, t_to, item0, T, run, lane, w, n, g);
   });

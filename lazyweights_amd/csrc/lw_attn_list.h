@@ -13,8 +13,9 @@ namespace lw {
 namespace {
 
 // Calls item(s, sequence, key-value head, row block, first key, first tile, end tile, item's first tile in the list, its
-// tiles, tiles of a run) for the tiles of every item that this block has. csum: [1024] in LDS.
-template <int NW, int KEYS, class Item>
+// tiles, tiles of a run) for the tiles of every item that this block has. csum: [1024] in LDS. WHOLE: a block may have an
+// item of its own (AttnArgs::whole).
+template <int NW, int KEYS, bool WHOLE, class Item>
 __device__ __forceinline__ void walk_items(const AttnArgs& a, uint32_t* csum, int lane, int w, Item&& item) {
   const KvView& c = a.c;
   const int seqs = c.seqs, kv_heads = c.kv_heads, H = kv_heads * a.row_blocks, chunks = (seqs + 63) >> 6;
@@ -22,7 +23,7 @@ __device__ __forceinline__ void walk_items(const AttnArgs& a, uint32_t* csum, in
   // the zeros
   auto first_key = [&](const Seq& q) { return a.window > 0 ? max(0, q.len - q.rows - a.window + 1) & ~(KEYS - 1) : 0; };
   auto tiles_of = [&](const Seq& q) { return q.rows ? max((q.len - first_key(q) + KEYS - 1) / KEYS, 1) : 0; };
-  if (a.whole) {
+  if (WHOLE && a.whole) {
     const int s = (int)blockIdx.x / H, hb = (int)blockIdx.x - s * H, rb = hb / kv_heads;
     const Seq sq = sequence(c, s);
     const int T = tiles_of(sq);

@@ -158,6 +158,10 @@ BATCHES = [
     ((32, 8, 128), 60, 900, 6000, 2),
     ((8, 4, 128), 300, 200, 4500, 1),
     ((16, 8, 128), 33, 5000, 5000, 1),
+    ((16, 8, 128), 20, 2500, 2500, 1),
+    ((32, 8, 128), 9, 900, 17000, 1),
+    # parts of a size
+    ((8, 8, 64), 28, 700, 9000, 1),
     # two row tiles in a block per item, in parts
     ((32, 4, 128), 130, 300, 600, 3),
     ((24, 4, 64), 300, 60, 2000, 5),
