@@ -99,9 +99,10 @@ __global__ __launch_bounds__(2 * D) void k_kv8_append(const Append8Args args, ui
   auto first_item = [&](int i, int from) { return clampi(from, 0, c.tokens) / kExpBlock + 2 * i; };
   int s = min((int)((int64_t)item * 16 / 33), c.seqs - 1);  // one new token per sequence first: 33 items for 16 of them
   const Seq sq = find(s, item, first_item);
-  const int past = sq.len - sq.rows, p0 = max(past, 0);
-  const int64_t block = (int64_t)p0 / kExpBlock + item - first_item(s, sq.row0);
-  if (sq.rows == 0 || block * kExpBlock >= sq.len) return;
+  // (items of no sequence: those before the first one's, whose rows may begin behind others)
+  const int past = sq.len - sq.rows, p0 = max(past, 0), nth = item - first_item(s, sq.row0);
+  const int64_t block = (int64_t)p0 / kExpBlock + nth;
+  if (sq.rows == 0 || nth < 0 || block * kExpBlock >= sq.len) return;
   const int begin = (int)block * kExpBlock, mask = (1 << c.page_shift) - 1;
   const int pos = begin + (int)threadIdx.x / U;
   const bool fresh = pos >= p0 && pos < sq.len, older = pos < p0, turn = 8 * unit < a.rot;
