@@ -82,19 +82,23 @@ class Sequences:
 
     def grow(self, news, q_start=None):
         """Room for news[s] more tokens of every sequence, in the tensors that the batches read; their rows' starts."""
-        self.lengths = [a + n for a, n in zip(self.lengths, news)]
-        if max(self.lengths) > self.most or sum(-(-n // self.page) for n in self.lengths) > self.pages.free.shape[0]:
-            raise RuntimeError("no pages left for %s tokens" % self.lengths)  # (known here without asking the GPU)
-        return self.pages.advance(torch.tensor(news, dtype=torch.int32, device="cuda"), rows=sum(news), q_start=q_start, places=False)[0]
+        lengths = [a + n for a, n in zip(self.lengths, news)]
+        if max(lengths) > self.most or sum(-(-n // self.page) for n in lengths) > self.pages.free.shape[0]:
+            raise RuntimeError("no pages left for %s tokens" % lengths)  # (known here without asking the GPU)
+        starts = self.pages.advance(torch.tensor(news, dtype=torch.int32, device="cuda"), rows=sum(news), q_start=q_start, places=False)[0]
+        self.lengths = lengths  # (a refused step leaves them, and its batch, as the GPU has them)
+        return starts
 
     def batch(self, news):
         """The batch in which every sequence has news[s] new tokens; the last KEPT kinds of them are kept, each with its workspace
         (steps of single tokens and drafts come again and again, prompts hardly ever in the same lengths; who captures a call keeps
         its batch)."""
         key = tuple(news)
-        batch = self.steady.pop(key, None)
+        batch = self.steady.get(key)
         starts = self.grow(news, batch and batch.tensors[0])
-        if batch is None:
+        if batch is not None:
+            del self.steady[key]
+        else:
             batch = Batch(self.layer.cache, self.layer.heads, starts, self.kv_len, self.table, max(news), self.most)
         self.steady[key] = batch  # (the last one used at the end)
         while len(self.steady) > self.KEPT:
