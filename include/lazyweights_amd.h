@@ -303,8 +303,8 @@ long long lw_attn8_workspace(const lw_kv8_cache* cache, const lw_batch* batch, i
  * for itself. A block's exponent is the least that holds the largest finite magnitude of its new rows (448 2^e at most, -48
  * for zeros), or what it was where the block has rows from before the call's first new one and that is more; where it
  * grows, those rows are rounded to it, once more. Numbers are rounded to nearest even; magnitudes past 448 2^48 are held as
- * that, infinities as NaN. Rows behind a sequence's last are left alone. A block is appended to by one sequence of a call: sequences
- * may share pages that are full, or that none of them appends to. */
+ * that, infinities as NaN. Rows behind a sequence's last are left alone. A block is appended to by one sequence of a call, at one place of
+ * its page table: sequences may share pages that are full, or that none of them appends to. */
 int lw_kv8_append(const lw_kv8_cache* cache, const lw_batch* batch, int heads, const void* q, const void* k, const void* v,
                   int x_type, long long ldq, long long ldk, long long ldv, const float* cos, const float* sin, int rot,
                   int rope_rows, int neighbours, void* q_out, int q_type, long long ldo, void* stream);
@@ -319,7 +319,8 @@ int lw_attn8_prompt(const lw_kv8_cache* cache, const lw_batch* batch, int heads,
 
 /* The pages of `seqs` sequences (up to 8192) and the pool of those that none has, on the GPU: position j of sequence s
  * lies in row j % page_size of page table[s * table_stride + j / page_size]; free[0 .. left[0]) are the pool's pages, a
- * stack, of `pages` at most. page_size is a power of two up to 65536. workspace: LW_PAGES_WORKSPACE bytes, zero before its first use;
+ * stack, of `pages` at most. A page belongs to one sequence: what a sequence gives back is taken again, whoever else's table names it.
+ * page_size is a power of two up to 65536. workspace: LW_PAGES_WORKSPACE bytes, zero before its first use;
  * calls leave it zero, and calls that share one must not overlap. */
 enum { LW_PAGES_WORKSPACE = 1088 };
 typedef struct lw_pages {

@@ -418,6 +418,9 @@ DecodePlan decode8_plan(int seqs, int kv_heads, int group, int head_dim, int max
   // / parts: 512 items of 500-16000 keys 144 / 148, of 8000 182 / 189, of 1500-3500 74 / 101, of 500-4000 62 / 75, 2048 of 1500-3500 235 /
   // 306; 248 of 500-16000 67 / 84, 192 of 1500-3500 29 / 33; 128 of 20000-60000 207 / 228, of 8000 60 / 61, of 1500-3500 24 / 23; but
   // 2048 of 100-2000 119 / 88. Heads of 96, whose tiles are smaller, need more waves beside one another: 512 of 500-16000 124 / 101.
+  // All of these with the longest length as the bound. The host knows bounds alone, and under a bound far above the lengths short items go in
+  // runs too: 512 items of 100-2000 keys 34 with a bound of 8192 and more, 25 of 2000; of 30-500 23 and 14; 2048 of 100-2000 113 and 86, of
+  // 200-800 62 and 44; 1024 of 300-1500 48 and 40 (1500-3500 are 62 with any).
   p.runs = !p.whole && p.row_tiles == 1 && head_dim == 128 && (items > 128 ? max_kv > 2048 : items >= 64 && max_kv > 16384);
   p.blocks_log2 = 9;
   // Parts: few items in about as many blocks as there are CUs (the more parts of an item, the longer its join: one of 131071 keys with

@@ -77,7 +77,8 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int tile) {
 // and then added to the rows' sums, and l by add_exactly(): what a weight's later parts add is near the last bit of a long sum,
 // and where many weights are alike every addition loses the same of it (40000 like keys: 4.3e-5 of the output without,
 // 1.3e-6 with). It takes an addition per sum and tile: 9000 tokens of 32 heads of 128 in fp16 1010 us against 982, 1000 tokens of 32
-// heads of 96 after 12000 375 against 303, so that shorter runs, whose sums have a few hundred steps a part, go without.
+// heads of 96 after 12000 375 against 303, so that shorter runs, whose sums have a few hundred steps a part, go without. (Over 8 bits,
+// heads of 128, and of 96 with 4 waves, have some of these sums' registers in memory within the loop; no other form of 8 bits has.)
 //
 // A cache in 8 bits (ARGS = Attn8Args): a wave's share of the tile after the next comes to registers while one is worked on, and goes to
 // LDS as 16-bit numbers, K's of q's type and V's fp16, which hold 8 bits exactly: converted once per block, since every wave reads all

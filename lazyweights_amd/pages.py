@@ -27,7 +27,8 @@ class _Pages(ctypes.Structure):
 class Pages:
     """Sequences' tables int32 [seqs, table_pages] and lengths kv_len int32 [seqs], and the free pages: free int32 [pages], a stack of
     which the first left[0] are free (left int32 [2]; left[1] says what the last step lacked: 0 nothing, else the sum of 1: pages, 2:
-    room in the table, 4: rows; then it has changed nothing). All on one GPU, contiguous (the table's rows may lie apart)."""
+    room in the table, 4: rows; then it has changed nothing). All on one GPU, contiguous (the table's rows may lie apart). A page belongs to
+    one sequence: what is given back is taken again, whoever else's table names it."""
 
     def __init__(self, page_size, kv_len, table, free, left):
         seqs = kv_len.shape[0] if kv_len.dim() == 1 else -1
